@@ -10,7 +10,7 @@
  *   - All tensor pointers are CUDA device pointers owned by the caller unless a name starts with
  *     h_.  `stream` is a cudaStream_t passed as void* (NULL = the legacy default stream).  Calls
  *     only enqueue work; ordering is the stream's (the reference returned cl_events instead).
- *   - dtype: SDFL_F32 or SDFL_F16 storage; arithmetic is always fp32; weights (gamma, beta) are
+ *   - dtype: SDFL_F32 or SDFL_F16 storage (SDFL_BF16 too where a section says so); arithmetic is always fp32; weights (gamma, beta) are
  *     always fp32, as in the reference.
  *   - Return value: 0 on success, a negative SDFL_ERR_* otherwise.  Nothing throws, nothing
  *     aborts.  The reference returned cl_int (0 = CL_SUCCESS) and threw std::runtime_error on
@@ -30,7 +30,8 @@
 extern "C" {
 #endif
 
-enum { SDFL_F32 = 0, SDFL_F16 = 1 };
+/* SDFL_BF16 is taken by the channels-last GroupNorm and the checkpoint entry points only. */
+enum { SDFL_F32 = 0, SDFL_F16 = 1, SDFL_BF16 = 2 };
 
 enum {
     SDFL_OK = 0,
@@ -343,6 +344,74 @@ int sdfl_quick_gelu(const void *src, void *dst, int64_t n, int dtype, void *stre
 
 /* K/util.cl:1-12  elemwise_add(A, B, C): C = A + B over n work-items. */
 int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtype, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Channels-last GroupNorm, its gradient, and 8-bit activation checkpoints (training)
+ *
+ * No counterpart in the reference (an inference app on NCHW buffers).  dtype here may also be
+ * SDFL_BF16; arithmetic, weights, statistics and weight gradients are fp32.
+ *
+ * Checkpoint format.  A tensor is seen as [rows, dim]; a row is cut into blocks of 32 consecutive
+ * elements, the last one of a row possibly shorter.  With a = max |x| of a block and
+ * e = floor(log2 a):  step = 2^max(e - 6, -120), code = x / step rounded to the nearest integer
+ * (ties to even) and clamped to [-127, 127]; the value kept is code * step.
+ *   codes  [rows, dim]            int8
+ *   scales [rows, ceil(dim / 32)] uint8, 127 + log2(step)
+ * That is 1 + 1/32 bytes per element.  |value - x| <= step / 2, or < step where |x| > 127.5 step; every value
+ * is exact in bf16, fp16 and fp32.  A block that holds an infinity or a NaN has scale 255 and
+ * codes 0 and expands to NaN throughout, so that the gradients show it.
+ * ---------------------------------------------------------------------------------------- */
+
+/* GroupNorm with optional fused SiLU on a channels-last tensor [batch, hw, channels]: group g of
+ * an image is channels [g*C/G, (g+1)*C/G) of all its pixels, biased variance, eps inside the square root, as in
+ * sdfl_groupnorm_forward.  out may be in.
+ * mean, rstd: NULL, or [batch, num_groups] fp32 that receive the statistics the backward pass
+ * needs (rstd = 1 / sqrt(variance + eps)).
+ * codes, scales: NULL, or a checkpoint of `in` seen as [batch * hw, channels], written in the same call.
+ * workspace: 16-byte aligned, sdfl_groupnorm_channels_last_workspace_bytes(..., backward = 0)
+ * bytes, contents of no matter; launches that can overlap on the GPU need one each (two captured
+ * graphs that hold the same workspace must not run at the same time).
+ * batch == 0 or hw == 0 writes nothing. */
+size_t sdfl_groupnorm_channels_last_workspace_bytes(int64_t batch, int64_t channels, int64_t hw,
+                                                    int64_t num_groups, int backward, int dtype);
+int sdfl_groupnorm_channels_last_forward(const void *in, void *out, const float *gamma, const float *beta,
+                                         float *mean, float *rstd, int8_t *codes, uint8_t *scales,
+                                         int64_t batch, int64_t channels, int64_t hw, int64_t num_groups,
+                                         float eps, int fuse_silu, int dtype, void *workspace,
+                                         size_t workspace_bytes, void *stream);
+
+/* Gradient of the call above.  The forward's input is given either as `in` (codes and scales
+ * NULL) or by its checkpoint (in NULL); both is SDFL_ERR_INVALID_VALUE.  With xhat = (x - mean) rstd,
+ * z = xhat gamma + beta, dz = grad_out act'(z):
+ *   grad_beta[c]  = sum dz,  grad_gamma[c] = sum dz xhat   over images and pixels
+ *   grad_in       = rstd (gamma dz - m1 - xhat m2),  m1, m2 = means of gamma dz and gamma dz xhat
+ *                   over the group's elements
+ * grad_gamma and grad_beta are [channels] fp32 and may be NULL; they are written, not added to.
+ * Sums run in a fixed order: the same inputs give the same bits.  grad_in may be `in` or grad_out.
+ * An empty tensor writes zeros to grad_gamma and grad_beta. */
+int sdfl_groupnorm_channels_last_backward(const void *in, const int8_t *codes, const uint8_t *scales,
+                                          const void *grad_out, void *grad_in, const float *gamma,
+                                          const float *beta, const float *mean, const float *rstd,
+                                          float *grad_gamma, float *grad_beta, int64_t batch,
+                                          int64_t channels, int64_t hw, int64_t num_groups, int fuse_silu,
+                                          int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* A checkpoint of [rows, dim], and its expansion to dtype. */
+int sdfl_checkpoint_pack(const void *in, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim,
+                         int dtype, void *stream);
+int sdfl_checkpoint_unpack(const int8_t *codes, const uint8_t *scales, void *out, int64_t rows,
+                           int64_t dim, int dtype, void *stream);
+
+/* sdfl_gelu_multiply that also writes a checkpoint of AB seen as [rows, 2 D]. */
+int sdfl_gelu_multiply_checkpoint(const void *AB, void *dst, int8_t *codes, uint8_t *scales, int64_t rows,
+                                  int64_t D, int dtype, void *stream);
+
+/* Gradient of sdfl_gelu_multiply from AB or from its checkpoint (the other NULL):
+ *   grad_AB[r, j] = grad_out[r, j] g Phi(g),   grad_AB[r, D + j] = grad_out[r, j] a (Phi(g) + g phi(g))
+ * with a = AB[r, j], g = AB[r, D + j].  grad_AB may be AB. */
+int sdfl_gelu_multiply_backward(const void *AB, const int8_t *codes, const uint8_t *scales,
+                                const void *grad_out, void *grad_AB, int64_t rows, int64_t D, int dtype,
+                                void *stream);
 
 /* ------------------------------------------------------------------------------------------
  * Operator objects: the reference's classes as opaque C handles, for binders that cannot use the

@@ -11,7 +11,7 @@ import os
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "lib", "libsdfl.so")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 GN_AUTO, GN_RESIDENT, GN_SPLIT, GN_REGISTER = 0, 1, 2, 3
 
 OK = 0
@@ -97,6 +97,15 @@ SIGNATURES = {
     "sdfl_geglu_weight_shape": (_i, [_p, C.POINTER(_i64)]),
     "sdfl_geglu_op_forward": (_i, [_p, _p, _p, _i64, _i, _p]),
     "sdfl_geglu_destroy": (_i, [_p]),
+    "sdfl_groupnorm_channels_last_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i, _i]),
+    "sdfl_groupnorm_channels_last_forward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f, _i, _i,
+                                                  _p, _sz, _p]),
+    "sdfl_groupnorm_channels_last_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                                                   _i, _i, _p, _sz, _p]),
+    "sdfl_checkpoint_pack": (_i, [_p, _p, _p, _i64, _i64, _i, _p]),
+    "sdfl_checkpoint_unpack": (_i, [_p, _p, _p, _i64, _i64, _i, _p]),
+    "sdfl_gelu_multiply_checkpoint": (_i, [_p, _p, _p, _p, _i64, _i64, _i, _p]),
+    "sdfl_gelu_multiply_backward": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i, _p]),
     "sdfl_device_status": (_i, [C.POINTER(C.c_uint), _i, _p]),
     "sdfl_selftest_bounded_wait": (_i, [C.c_longlong, _p]),
     "sdfl_host_pipeline_create": (_i, [C.POINTER(_p), _sz, _i]),

@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "kernels.h"
 
+#include <initializer_list>
 #include <new>
 #include <vector>
 
@@ -74,6 +75,36 @@ int gn_forward(const void *in, void *out, const float *gamma, const float *beta,
     if (plan.path == sdfl::kGnSplit && (workspace == nullptr || workspace_bytes < plan.workspace))
         return SDFL_ERR_WORKSPACE;
     return wrap(sdfl::gn_launch(s, plan, in, out, gamma, beta, workspace, stream, bias));
+}
+
+// ---- channels-last GroupNorm and checkpoints: these also take bf16 ---------------------------------
+inline bool train_dtype_ok(int dtype) { return dtype_ok(dtype) || dtype == SDFL_BF16; }
+inline int64_t train_esize(int dtype) { return dtype == SDFL_F32 ? 4 : 2; }
+
+int gn_cl_validate(const void *in, const void *out, const float *gamma, const float *beta, int64_t batch,
+                   int64_t channels, int64_t hw, int64_t groups, float eps, int dtype) {
+    if (!train_dtype_ok(dtype)) return SDFL_ERR_INVALID_VALUE;
+    // bf16 has fp16's size, which is all that the checks look at
+    return gn_validate(in, out, gamma, beta, batch, channels, hw, groups, eps,
+                       dtype == SDFL_F32 ? SDFL_F32 : SDFL_F16);
+}
+
+// A checkpoint's two arrays: both or neither; true if either touches [p, p + bytes).
+inline bool ckpt_half(const void *codes, const void *scales) { return (codes == nullptr) != (scales == nullptr); }
+inline int64_t ckpt_scale_bytes(int64_t rows, int64_t dim) { return rows * ((dim + 31) / 32); }
+inline bool ckpt_overlaps(const void *codes, const void *scales, int64_t rows, int64_t dim, const void *p, int64_t bytes) {
+    return any_overlap(codes, rows * dim, p, bytes) || any_overlap(scales, ckpt_scale_bytes(rows, dim), p, bytes);
+}
+inline int ckpt_shape_check(int64_t rows, int64_t dim, int dtype) {
+    if (!train_dtype_ok(dtype) || rows < 0 || dim < 0) return SDFL_ERR_INVALID_VALUE;
+    if (dim >= (1ll << 31) || rows >= (1ll << 40)) return SDFL_ERR_UNSUPPORTED;
+    return SDFL_OK;
+}
+
+inline int workspace_check(const void *workspace, size_t have, size_t need) {
+    if (need == 0) return SDFL_OK;
+    if (!workspace || have < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return SDFL_ERR_WORKSPACE;
+    return SDFL_OK;
 }
 
 int unary(int act, const void *src, void *dst, int64_t n, int dtype, void *stream) {
@@ -536,6 +567,128 @@ int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtyp
     if (partial_overlap(A, bytes, C, bytes) || partial_overlap(B, bytes, C, bytes))
         return SDFL_ERR_OVERLAP;
     return wrap(sdfl::add_launch(A, B, C, n, dtype, as_stream(stream)));
+}
+
+// ---- channels-last GroupNorm, 8-bit activation checkpoints and the gradients that read them ---------
+
+size_t sdfl_groupnorm_channels_last_workspace_bytes(int64_t batch, int64_t channels, int64_t hw, int64_t num_groups,
+                                                    int backward, int dtype) {
+    if (!train_dtype_ok(dtype) || batch <= 0 || channels <= 0 || hw <= 0 || num_groups <= 0 ||
+        channels % num_groups != 0)
+        return 0;
+    sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, 0.f, sdfl::kActNone};
+    return sdfl::gn_cl_workspace_bytes(s, backward != 0);
+}
+
+int sdfl_groupnorm_channels_last_forward(const void *in, void *out, const float *gamma, const float *beta, float *mean,
+                                         float *rstd, int8_t *codes, uint8_t *scales, int64_t batch, int64_t channels,
+                                         int64_t hw, int64_t num_groups, float eps, int fuse_silu, int dtype,
+                                         void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = gn_cl_validate(in, out, gamma, beta, batch, channels, hw, num_groups, eps, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (batch == 0 || hw == 0) return SDFL_OK;
+    if ((mean == nullptr) != (rstd == nullptr) || ckpt_half(codes, scales)) return SDFL_ERR_INVALID_POINTER;
+    const int64_t bytes = batch * channels * hw * train_esize(dtype), sums = batch * num_groups * 4;
+    if (mean && (any_overlap(mean, sums, out, bytes) || any_overlap(rstd, sums, out, bytes) ||
+                 any_overlap(mean, sums, in, bytes) || any_overlap(rstd, sums, in, bytes) ||
+                 any_overlap(mean, sums, rstd, sums)))
+        return SDFL_ERR_OVERLAP;
+    if (codes && (ckpt_overlaps(codes, scales, batch * hw, channels, in, bytes) ||
+                  ckpt_overlaps(codes, scales, batch * hw, channels, out, bytes) ||
+                  any_overlap(codes, batch * hw * channels, scales, ckpt_scale_bytes(batch * hw, channels))))
+        return SDFL_ERR_OVERLAP;
+    sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, eps, fuse_silu ? sdfl::kActSilu : sdfl::kActNone};
+    rc = workspace_check(workspace, workspace_bytes, sdfl::gn_cl_workspace_bytes(s, false));
+    if (rc != SDFL_OK) return rc;
+    sdfl::GnClForward a{in, out, gamma, beta, mean, rstd, codes, scales};
+    cudaError_t e = sdfl::gn_cl_forward_launch(s, a, workspace, as_stream(stream));
+    if (e == cudaErrorInvalidConfiguration) return SDFL_ERR_UNSUPPORTED;
+    return wrap(e);
+}
+
+int sdfl_groupnorm_channels_last_backward(const void *in, const int8_t *codes, const uint8_t *scales, const void *grad_out,
+                                          void *grad_in, const float *gamma, const float *beta, const float *mean,
+                                          const float *rstd, float *grad_gamma, float *grad_beta, int64_t batch,
+                                          int64_t channels, int64_t hw, int64_t num_groups, int fuse_silu, int dtype,
+                                          void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = gn_cl_validate(grad_out, grad_in, gamma, beta, batch, channels, hw, num_groups, 0.f, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (batch == 0 || hw == 0) {                        // sums over nothing
+        cudaError_t e = cudaSuccess;
+        if (grad_gamma) e = cudaMemsetAsync(grad_gamma, 0, channels * sizeof(float), as_stream(stream));
+        if (e == cudaSuccess && grad_beta)
+            e = cudaMemsetAsync(grad_beta, 0, channels * sizeof(float), as_stream(stream));
+        return wrap(e);
+    }
+    if (ckpt_half(codes, scales) || !mean || !rstd || (!in && !codes)) return SDFL_ERR_INVALID_POINTER;
+    if (in && codes) return SDFL_ERR_INVALID_VALUE;      // one source
+    const int64_t bytes = batch * channels * hw * train_esize(dtype);
+    if (in && partial_overlap(in, bytes, grad_in, bytes)) return SDFL_ERR_OVERLAP;
+    if (codes && ckpt_overlaps(codes, scales, batch * hw, channels, grad_in, bytes)) return SDFL_ERR_OVERLAP;
+    const int64_t params = channels * 4;
+    for (const float *p : {grad_gamma, grad_beta})
+        if (p && (any_overlap(p, params, grad_in, bytes) || any_overlap(p, params, grad_out, bytes) ||
+                  (in && any_overlap(p, params, in, bytes)) || any_overlap(p, params, gamma, params) ||
+                  any_overlap(p, params, beta, params)))
+            return SDFL_ERR_OVERLAP;
+    if (grad_gamma && grad_beta && any_overlap(grad_gamma, params, grad_beta, params)) return SDFL_ERR_OVERLAP;
+    sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, 0.f, fuse_silu ? sdfl::kActSilu : sdfl::kActNone};
+    rc = workspace_check(workspace, workspace_bytes, sdfl::gn_cl_workspace_bytes(s, true));
+    if (rc != SDFL_OK) return rc;
+    sdfl::GnClBackward a{in, codes, scales, grad_out, grad_in, gamma, beta, mean, rstd, grad_gamma, grad_beta};
+    cudaError_t e = sdfl::gn_cl_backward_launch(s, a, workspace, as_stream(stream));
+    if (e == cudaErrorInvalidConfiguration) return SDFL_ERR_UNSUPPORTED;
+    return wrap(e);
+}
+
+int sdfl_checkpoint_pack(const void *in, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim, int dtype,
+                         void *stream) {
+    int rc = ckpt_shape_check(rows, dim, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (rows == 0 || dim == 0) return SDFL_OK;
+    if (!in || !codes || !scales) return SDFL_ERR_INVALID_POINTER;
+    if (ckpt_overlaps(codes, scales, rows, dim, in, rows * dim * train_esize(dtype)) ||
+        any_overlap(codes, rows * dim, scales, ckpt_scale_bytes(rows, dim)))
+        return SDFL_ERR_OVERLAP;
+    return wrap(sdfl::ckpt_pack_launch(in, codes, scales, rows, dim, dtype, as_stream(stream)));
+}
+
+int sdfl_checkpoint_unpack(const int8_t *codes, const uint8_t *scales, void *out, int64_t rows, int64_t dim, int dtype,
+                           void *stream) {
+    int rc = ckpt_shape_check(rows, dim, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (rows == 0 || dim == 0) return SDFL_OK;
+    if (!out || !codes || !scales) return SDFL_ERR_INVALID_POINTER;
+    if (ckpt_overlaps(codes, scales, rows, dim, out, rows * dim * train_esize(dtype))) return SDFL_ERR_OVERLAP;
+    return wrap(sdfl::ckpt_unpack_launch(codes, scales, out, rows, dim, dtype, as_stream(stream)));
+}
+
+int sdfl_gelu_multiply_checkpoint(const void *AB, void *dst, int8_t *codes, uint8_t *scales, int64_t rows, int64_t D,
+                                  int dtype, void *stream) {
+    int rc = ckpt_shape_check(rows, D, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (rows == 0 || D == 0) return SDFL_OK;
+    if (!AB || !dst || !codes || !scales) return SDFL_ERR_INVALID_POINTER;
+    const int64_t out = rows * D * train_esize(dtype);
+    if (any_overlap(AB, 2 * out, dst, out) || ckpt_overlaps(codes, scales, rows, 2 * D, AB, 2 * out) ||
+        ckpt_overlaps(codes, scales, rows, 2 * D, dst, out) ||
+        any_overlap(codes, 2 * rows * D, scales, ckpt_scale_bytes(rows, 2 * D)))
+        return SDFL_ERR_OVERLAP;
+    return wrap(sdfl::geglu_pack_launch(AB, dst, codes, scales, rows, D, dtype, as_stream(stream)));
+}
+
+int sdfl_gelu_multiply_backward(const void *AB, const int8_t *codes, const uint8_t *scales, const void *grad_out,
+                                void *grad_AB, int64_t rows, int64_t D, int dtype, void *stream) {
+    int rc = ckpt_shape_check(rows, D, dtype);
+    if (rc != SDFL_OK) return rc;
+    if (rows == 0 || D == 0) return SDFL_OK;
+    if (ckpt_half(codes, scales) || !grad_out || !grad_AB || (!AB && !codes)) return SDFL_ERR_INVALID_POINTER;
+    if (AB && codes) return SDFL_ERR_INVALID_VALUE;      // one source
+    const int64_t out = rows * D * train_esize(dtype);
+    if (any_overlap(grad_out, out, grad_AB, 2 * out) || (AB && partial_overlap(AB, 2 * out, grad_AB, 2 * out)) ||
+        (codes && ckpt_overlaps(codes, scales, rows, 2 * D, grad_AB, 2 * out)))
+        return SDFL_ERR_OVERLAP;
+    return wrap(sdfl::geglu_backward_launch(AB, codes, scales, grad_out, grad_AB, rows, D, dtype, as_stream(stream)));
 }
 
 int sdfl_device_status(unsigned int *value, int clear, void *stream) {

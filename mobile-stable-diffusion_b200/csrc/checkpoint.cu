@@ -1,0 +1,392 @@
+// 8-bit activation checkpoints (format: ckpt_device.cuh): packing and expanding, the GEGLU gate that
+// keeps a checkpoint of its input, and the gate's backward pass from the whole input or from the
+// checkpoint.  fp32, fp16 or bf16 storage, fp32 arithmetic.
+//
+// Every kernel is one pass, bounded by HBM: bytes per element of the input of size s are
+// s + 33/32 (pack, expand), and per gate element 3 s + 2 * 33/32 (forward with checkpoint),
+// 5 s or 3 s + 2 * 33/32 (backward).
+//
+// Vector kernels: one thread per 16-byte vector (8 or 4 elements), so a block of 32 is 4 or 8
+// neighbouring lanes and its maximum is 2 or 3 shuffles.  They need 16-byte aligned buffers and
+// rows that are whole vectors; rows that are not whole blocks are walked as if padded to whole
+// blocks, the lanes beyond the row end idle.  Everything else takes the element kernels, one
+// lane per element and one warp per block of 32.
+#include "ckpt_device.cuh"
+#include "kernels.h"
+
+namespace sdfl {
+
+namespace {
+
+constexpr int kCkThreads = 256;
+
+inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+inline unsigned ck_grid(int64_t work_items) {
+    int64_t blocks = (work_items + kCkThreads - 1) / kCkThreads;
+    const int64_t cap = static_cast<int64_t>(sm_count()) * 8 * 4;
+    if (blocks > cap) blocks = cap;
+    if (blocks < 1) blocks = 1;
+    return static_cast<unsigned>(blocks);
+}
+
+// ---- pack ---------------------------------------------------------------------------------------
+// A slot is one vector of a row padded to whole blocks.  RAGGED = false: rows are whole blocks, a slot
+// is a vector of the flat tensor.
+template <typename T, bool RAGGED>
+__global__ void __launch_bounds__(kCkThreads)
+pack_vec_kernel(const uint4 *__restrict__ src, typename CodeVec<VecOf<T>::N>::type *__restrict__ codes,
+                uint8_t *__restrict__ scales, long long nslots, uint32_t slots_row, FastDiv slots_div, uint32_t vecs_row) {
+    constexpr int VEC = VecOf<T>::N;
+    constexpr int LANES = kCkptBlock / VEC;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    // whole warps go round together: the shuffles need every lane
+    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads + (threadIdx.x & ~31); base < nslots;
+         base += stride) {
+        const long long i = base + (threadIdx.x & 31);
+        long long at = i;
+        bool live = i < nslots;
+        if (RAGGED) {
+            const uint32_t row = slots_div.div(static_cast<uint32_t>(i));
+            const uint32_t col = static_cast<uint32_t>(i) - row * slots_row;
+            live = live && col < vecs_row;
+            at = static_cast<long long>(row) * vecs_row + col;
+        }
+        float f[VEC];
+        unpack<T>(live ? ld_stream(src + at) : make_uint4(0, 0, 0, 0), f);
+        const CkptScale s = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
+        if (live) {
+            codes[at] = ckpt_codes(f, s);
+            if ((threadIdx.x & (LANES - 1)) == 0) scales[i / LANES] = static_cast<uint8_t>(s.e);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kCkThreads)
+pack_element_kernel(const T *__restrict__ src, int8_t *__restrict__ codes, uint8_t *__restrict__ scales,
+                    long long nblocks, long long dim, long long blocks_row) {
+    const int lane = threadIdx.x & 31;
+    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32);
+    for (long long b = static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); b < nblocks;
+         b += stride) {
+        const long long row = b / blocks_row, col = (b - row * blocks_row) * kCkptBlock + lane;
+        const bool live = col < dim;
+        const float x = live ? to_float<T>(src[row * dim + col]) : 0.f;
+        const CkptScale s = ckpt_scale(__reduce_max_sync(0xffffffffu, abs_bits(x)));
+        if (live) codes[row * dim + col] = static_cast<int8_t>(ckpt_code(x, s.inv) & s.keep);
+        if (lane == 0) scales[b] = static_cast<uint8_t>(s.e);
+    }
+}
+
+template <typename T>
+cudaError_t pack_dispatch(const void *src, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim,
+                          cudaStream_t stream) {
+    constexpr int VEC = VecOf<T>::N;
+    using CV = typename CodeVec<VEC>::type;
+    const int64_t blocks_row = ckpt_blocks(dim), nblocks = rows * blocks_row;
+    const int64_t slots_row = blocks_row * (kCkptBlock / VEC), nslots = rows * slots_row;
+    const bool vec = dim % VEC == 0 && aligned(src, 16) && aligned(codes, VEC);
+    if (vec && dim % kCkptBlock == 0) {
+        pack_vec_kernel<T, false><<<ck_grid(nslots), kCkThreads, 0, stream>>>(
+            static_cast<const uint4 *>(src), reinterpret_cast<CV *>(codes), scales, nslots, 1, FastDiv::make(1), 1);
+    } else if (vec && nslots < (1ll << 31)) {
+        pack_vec_kernel<T, true><<<ck_grid(nslots), kCkThreads, 0, stream>>>(
+            static_cast<const uint4 *>(src), reinterpret_cast<CV *>(codes), scales, nslots,
+            static_cast<uint32_t>(slots_row), FastDiv::make(static_cast<uint32_t>(slots_row)),
+            static_cast<uint32_t>(dim / VEC));
+    } else {
+        pack_element_kernel<T><<<ck_grid(nblocks * 32), kCkThreads, 0, stream>>>(static_cast<const T *>(src), codes, scales,
+                                                                                nblocks, dim, blocks_row);
+    }
+    cudaError_t err = cudaGetLastError();
+    if (err == cudaSuccess) g_launches.fetch_add(1);
+    return err;
+}
+
+// ---- expand -------------------------------------------------------------------------------------
+template <typename T, bool RAGGED>
+__global__ void __launch_bounds__(kCkThreads)
+unpack_vec_kernel(const typename CodeVec<VecOf<T>::N>::type *__restrict__ codes, const uint8_t *__restrict__ scales,
+                  uint4 *__restrict__ dst, long long nvec, uint32_t vecs_row, FastDiv vecs_div, uint32_t blocks_row) {
+    constexpr int VEC = VecOf<T>::N;
+    constexpr int LANES = kCkptBlock / VEC;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < nvec; i += stride) {
+        long long block = i / LANES;
+        if (RAGGED) {
+            const uint32_t row = vecs_div.div(static_cast<uint32_t>(i));
+            const uint32_t col = static_cast<uint32_t>(i) - row * vecs_row;
+            block = static_cast<long long>(row) * blocks_row + col / LANES;
+        }
+        float f[VEC];
+        ckpt_values(__ldcs(codes + i), ckpt_step(__ldg(scales + block)), f);
+        st_stream(dst + i, pack<T>(f));
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kCkThreads)
+unpack_element_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales, T *__restrict__ dst,
+                      long long nblocks, long long dim, long long blocks_row) {
+    const int lane = threadIdx.x & 31;
+    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32);
+    for (long long b = static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); b < nblocks;
+         b += stride) {
+        const long long row = b / blocks_row, col = (b - row * blocks_row) * kCkptBlock + lane;
+        if (col < dim) dst[row * dim + col] = from_float<T>(ckpt_value(codes[row * dim + col], scales[b]));
+    }
+}
+
+template <typename T>
+cudaError_t unpack_dispatch(const int8_t *codes, const uint8_t *scales, void *dst, int64_t rows, int64_t dim,
+                            cudaStream_t stream) {
+    constexpr int VEC = VecOf<T>::N;
+    using CV = typename CodeVec<VEC>::type;
+    const int64_t blocks_row = ckpt_blocks(dim), nblocks = rows * blocks_row;
+    const int64_t vecs_row = dim / VEC, nvec = rows * vecs_row;
+    const bool vec = dim % VEC == 0 && aligned(dst, 16) && aligned(codes, VEC);
+    if (vec && dim % kCkptBlock == 0) {
+        unpack_vec_kernel<T, false><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+            reinterpret_cast<const CV *>(codes), scales, static_cast<uint4 *>(dst), nvec, 1, FastDiv::make(1), 1);
+    } else if (vec && nvec < (1ll << 31)) {
+        unpack_vec_kernel<T, true><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+            reinterpret_cast<const CV *>(codes), scales, static_cast<uint4 *>(dst), nvec, static_cast<uint32_t>(vecs_row),
+            FastDiv::make(static_cast<uint32_t>(vecs_row)), static_cast<uint32_t>(blocks_row));
+    } else {
+        unpack_element_kernel<T><<<ck_grid(nblocks * 32), kCkThreads, 0, stream>>>(codes, scales, static_cast<T *>(dst),
+                                                                                  nblocks, dim, blocks_row);
+    }
+    cudaError_t err = cudaGetLastError();
+    if (err == cudaSuccess) g_launches.fetch_add(1);
+    return err;
+}
+
+// ---- GEGLU gate with a checkpoint of its input [rows, 2 D] -----------------------------------------
+// D a multiple of 32, so that no block holds elements of both halves.  The gate itself is the
+// arithmetic of gelu_multiply: the same bits come out.
+template <typename T>
+__global__ void __launch_bounds__(kCkThreads)
+geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
+                  typename CodeVec<VecOf<T>::N>::type *__restrict__ codes, uint8_t *__restrict__ scales,
+                  long long nvec, FastDiv dvec_div, uint32_t dvec) {
+    constexpr int VEC = VecOf<T>::N;
+    constexpr int LANES = kCkptBlock / VEC;
+    constexpr bool HALF = sizeof(T) == 2;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads + (threadIdx.x & ~31); base < nvec;
+         base += stride) {
+        const long long i = base + (threadIdx.x & 31);
+        const bool live = i < nvec;
+        const uint32_t r = dvec_div.div(static_cast<uint32_t>(live ? i : 0));
+        const uint32_t j = static_cast<uint32_t>(live ? i : 0) - r * dvec;
+        const long long at = static_cast<long long>(r) * 2 * dvec + j;
+        float a[VEC], g[VEC];
+        unpack<T>(live ? ld_stream(ab + at) : make_uint4(0, 0, 0, 0), a);
+        unpack<T>(live ? ld_stream(ab + at + dvec) : make_uint4(0, 0, 0, 0), g);
+        const CkptScale sa = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(a)));
+        const CkptScale sg = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(g)));
+        if (live) {
+            codes[at] = ckpt_codes(a, sa);
+            codes[at + dvec] = ckpt_codes(g, sg);
+            if ((threadIdx.x & (LANES - 1)) == 0) {
+                scales[at / LANES] = static_cast<uint8_t>(sa.e);
+                scales[(at + dvec) / LANES] = static_cast<uint8_t>(sg.e);
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) a[k] = a[k] * gelu_erf<HALF>(g[k]);
+            st_stream(dst + i, pack<T>(a));
+        }
+    }
+}
+
+// The gate alone, element by element: with pack_dispatch the two-launch form for shapes that the
+// fused kernel does not take.
+template <typename T>
+__global__ void __launch_bounds__(kCkThreads)
+geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, long long rows, long long d) {
+    constexpr bool HALF = sizeof(T) == 2;
+    const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
+        const long long r = i / d, j = i - r * d;
+        dst[i] = from_float<T>(to_float<T>(ab[r * 2 * d + j]) * gelu_erf<HALF>(to_float<T>(ab[r * 2 * d + d + j])));
+    }
+}
+
+template <typename T>
+cudaError_t geglu_pack_dispatch(const void *ab, void *dst, int8_t *codes, uint8_t *scales, int64_t rows, int64_t d,
+                                cudaStream_t stream) {
+    constexpr int VEC = VecOf<T>::N;
+    using CV = typename CodeVec<VEC>::type;
+    const int64_t nvec = rows * (d / VEC);
+    if (d % kCkptBlock == 0 && aligned(ab, 16) && aligned(dst, 16) && aligned(codes, VEC) && nvec < (1ll << 31)) {
+        const uint32_t dvec = static_cast<uint32_t>(d / VEC);
+        geglu_pack_kernel<T><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+            static_cast<const uint4 *>(ab), static_cast<uint4 *>(dst), reinterpret_cast<CV *>(codes), scales, nvec,
+            FastDiv::make(dvec), dvec);
+        cudaError_t err = cudaGetLastError();
+        if (err == cudaSuccess) g_launches.fetch_add(1);
+        return err;
+    }
+    geglu_element_kernel<T><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(static_cast<const T *>(ab), static_cast<T *>(dst),
+                                                                          rows, d);
+    cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+    g_launches.fetch_add(1);
+    return pack_dispatch<T>(ab, codes, scales, rows, 2 * d, stream);
+}
+
+// ---- backward of the gate -----------------------------------------------------------------------
+// y = a gelu(g), gelu(g) = g Phi(g):  da = dy g Phi(g),  dg = dy a (Phi(g) + g phi(g)).
+// Phi for half storage from the same rational approximation as the forward's erf, taken as the tail
+// probability first (no cancellation for negative g); phi shares its exponential.  fp32 storage uses erfcf.
+template <bool HALF> __device__ __forceinline__ void gelu_grad(float g, float *value, float *slope) {
+    float cdf, pdf;
+    if (HALF) {
+        const float ax = fabsf(g) * 0.70710678118654752440f;
+        const float t = rcp_approx(fmaf(0.3275911f, ax, 1.0f));
+        float p = fmaf(1.061405429f, t, -1.453152027f);
+        p = fmaf(p, t, 1.421413741f);
+        p = fmaf(p, t, -0.284496736f);
+        p = fmaf(p, t, 0.254829592f);
+        const float e = ex2_approx(-1.4426950408889634f * ax * ax);
+        const float tail = 0.5f * p * t * e;
+        cdf = g < 0.f ? tail : 1.0f - tail;
+        pdf = e * 0.39894228040143267794f;
+    } else {
+        cdf = 0.5f * erfcf(g * -0.70710678118654752440f);
+        pdf = expf(-0.5f * g * g) * 0.39894228040143267794f;
+    }
+    *value = g * cdf;
+    *slope = fmaf(g, pdf, cdf);
+}
+
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(kCkThreads)
+geglu_backward_vec_kernel(const uint4 *ab, const typename CodeVec<VecOf<T>::N>::type *__restrict__ codes,
+                          const uint8_t *__restrict__ scales, const uint4 *dy, uint4 *dab, long long nvec,
+                          FastDiv dvec_div, uint32_t dvec, uint32_t blocks_row) {
+    constexpr int VEC = VecOf<T>::N;
+    constexpr int LANES = kCkptBlock / VEC;
+    constexpr bool HALF = sizeof(T) == 2;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < nvec; i += stride) {
+        const uint32_t r = dvec_div.div(static_cast<uint32_t>(i));
+        const uint32_t j = static_cast<uint32_t>(i) - r * dvec;
+        const long long at = static_cast<long long>(r) * 2 * dvec + j;
+        float a[VEC], g[VEC], d[VEC];
+        if (CKPT) {
+            const uint8_t *row = scales + static_cast<long long>(r) * blocks_row;
+            const auto ca = __ldcs(codes + at), cg = __ldcs(codes + at + dvec);
+            ckpt_values(ca, ckpt_step(__ldg(row + j / LANES)), a);
+            ckpt_values(cg, ckpt_step(__ldg(row + (j + dvec) / LANES)), g);
+        } else {
+            const uint4 va = ld_stream(ab + at), vg = ld_stream(ab + at + dvec);
+            unpack<T>(va, a);
+            unpack<T>(vg, g);
+        }
+        unpack<T>(ld_stream(dy + i), d);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            float value, slope;
+            gelu_grad<HALF>(g[k], &value, &slope);
+            g[k] = d[k] * a[k] * slope;
+            a[k] = d[k] * value;
+        }
+        st_stream(dab + at, pack<T>(a));
+        st_stream(dab + at + dvec, pack<T>(g));
+    }
+}
+
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(kCkThreads)
+geglu_backward_element_kernel(const T *ab, const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                              const T *dy, T *dab, long long rows, long long d, long long blocks_row) {
+    constexpr bool HALF = sizeof(T) == 2;
+    const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
+        const long long r = i / d, j = i - r * d, at = r * 2 * d + j;
+        float a, g;
+        if (CKPT) {
+            a = ckpt_value(codes[at], scales[r * blocks_row + j / kCkptBlock]);
+            g = ckpt_value(codes[at + d], scales[r * blocks_row + (j + d) / kCkptBlock]);
+        } else {
+            a = to_float<T>(ab[at]);
+            g = to_float<T>(ab[at + d]);
+        }
+        const float dyi = to_float<T>(dy[i]);
+        float value, slope;
+        gelu_grad<HALF>(g, &value, &slope);
+        dab[at] = from_float<T>(dyi * value);
+        dab[at + d] = from_float<T>(dyi * a * slope);
+    }
+}
+
+template <typename T, bool CKPT>
+cudaError_t geglu_backward_dispatch(const void *ab, const int8_t *codes, const uint8_t *scales, const void *dy, void *dab,
+                                    int64_t rows, int64_t d, cudaStream_t stream) {
+    constexpr int VEC = VecOf<T>::N;
+    using CV = typename CodeVec<VEC>::type;
+    const int64_t nvec = rows * (d / VEC), blocks_row = ckpt_blocks(2 * d);
+    const bool src_ok = CKPT ? aligned(codes, VEC) : aligned(ab, 16);
+    if (d % VEC == 0 && src_ok && aligned(dy, 16) && aligned(dab, 16) && nvec < (1ll << 31)) {
+        const uint32_t dvec = static_cast<uint32_t>(d / VEC);
+        geglu_backward_vec_kernel<T, CKPT><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+            static_cast<const uint4 *>(ab), reinterpret_cast<const CV *>(codes), scales, static_cast<const uint4 *>(dy),
+            static_cast<uint4 *>(dab), nvec, FastDiv::make(dvec), dvec, static_cast<uint32_t>(blocks_row));
+    } else {
+        geglu_backward_element_kernel<T, CKPT><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+            static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab), rows, d,
+            blocks_row);
+    }
+    cudaError_t err = cudaGetLastError();
+    if (err == cudaSuccess) g_launches.fetch_add(1);
+    return err;
+}
+
+template <typename T>
+cudaError_t geglu_backward_source(const void *ab, const int8_t *codes, const uint8_t *scales, const void *dy, void *dab,
+                                  int64_t rows, int64_t d, cudaStream_t stream) {
+    return codes ? geglu_backward_dispatch<T, true>(ab, codes, scales, dy, dab, rows, d, stream)
+                 : geglu_backward_dispatch<T, false>(ab, codes, scales, dy, dab, rows, d, stream);
+}
+
+}  // namespace
+
+cudaError_t ckpt_pack_launch(const void *src, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim, int dtype,
+                             cudaStream_t stream) {
+    switch (dtype) {
+        case kF16: return pack_dispatch<__half>(src, codes, scales, rows, dim, stream);
+        case kBF16: return pack_dispatch<__nv_bfloat16>(src, codes, scales, rows, dim, stream);
+        default: return pack_dispatch<float>(src, codes, scales, rows, dim, stream);
+    }
+}
+
+cudaError_t ckpt_unpack_launch(const int8_t *codes, const uint8_t *scales, void *dst, int64_t rows, int64_t dim, int dtype,
+                               cudaStream_t stream) {
+    switch (dtype) {
+        case kF16: return unpack_dispatch<__half>(codes, scales, dst, rows, dim, stream);
+        case kBF16: return unpack_dispatch<__nv_bfloat16>(codes, scales, dst, rows, dim, stream);
+        default: return unpack_dispatch<float>(codes, scales, dst, rows, dim, stream);
+    }
+}
+
+cudaError_t geglu_pack_launch(const void *ab, void *dst, int8_t *codes, uint8_t *scales, int64_t rows, int64_t d,
+                              int dtype, cudaStream_t stream) {
+    switch (dtype) {
+        case kF16: return geglu_pack_dispatch<__half>(ab, dst, codes, scales, rows, d, stream);
+        case kBF16: return geglu_pack_dispatch<__nv_bfloat16>(ab, dst, codes, scales, rows, d, stream);
+        default: return geglu_pack_dispatch<float>(ab, dst, codes, scales, rows, d, stream);
+    }
+}
+
+cudaError_t geglu_backward_launch(const void *ab, const int8_t *codes, const uint8_t *scales, const void *dy, void *dab,
+                                  int64_t rows, int64_t d, int dtype, cudaStream_t stream) {
+    switch (dtype) {
+        case kF16: return geglu_backward_source<__half>(ab, codes, scales, dy, dab, rows, d, stream);
+        case kBF16: return geglu_backward_source<__nv_bfloat16>(ab, codes, scales, dy, dab, rows, d, stream);
+        default: return geglu_backward_source<float>(ab, codes, scales, dy, dab, rows, d, stream);
+    }
+}
+
+}  // namespace sdfl

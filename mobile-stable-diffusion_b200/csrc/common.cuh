@@ -1,6 +1,7 @@
 // Shared device helpers for the fused-layer kernels (sm_100a only).
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -9,6 +10,7 @@ namespace sdfl {
 
 constexpr int kF32 = 0;
 constexpr int kF16 = 1;
+constexpr int kBF16 = 2;      // the channels-last and checkpoint kernels only
 
 enum Act : int { kActNone = 0, kActSilu = 1, kActGelu = 2, kActQuickGelu = 3 };
 
@@ -39,6 +41,7 @@ inline int sm_count() {
 template <typename T> struct VecOf;
 template <> struct VecOf<float> { static constexpr int N = 4; };
 template <> struct VecOf<__half> { static constexpr int N = 8; };
+template <> struct VecOf<__nv_bfloat16> { static constexpr int N = 8; };
 
 template <typename T> __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[VecOf<T>::N]);
 
@@ -57,6 +60,15 @@ template <> __device__ __forceinline__ void unpack<__half>(const uint4 &v, float
     }
 }
 
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4 &v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
 template <typename T> __device__ __forceinline__ uint4 pack(const float (&f)[VecOf<T>::N]);
 
 template <> __device__ __forceinline__ uint4 pack<float>(const float (&f)[4]) {
@@ -72,13 +84,24 @@ template <> __device__ __forceinline__ uint4 pack<__half>(const float (&f)[8]) {
     return v;
 }
 
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float (&f)[8]) {
+    uint4 v;
+    __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);   // RNE
+    return v;
+}
+
 template <typename T> __device__ __forceinline__ float to_float(T x);
 template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // Streaming 16-byte global accesses: the tensors here are touched once per launch.
 __device__ __forceinline__ uint4 ld_stream(const void *p) {

@@ -127,6 +127,46 @@ cudaError_t ln_apply_launch(const void *in, const float *mean, const float *var,
                             const float *b, int64_t dim, float eps, void *out, int64_t n, int dtype,
                             cudaStream_t stream);
 
+// ---- GroupNorm (+SiLU) of channels-last tensors [batch, hw, channels], and its gradient (gn_cl*.cu) ---
+struct GnClShape {
+    int64_t batch, channels, hw, groups;
+    int dtype;         // kF32 / kF16 / kBF16
+    float eps;
+    int act;           // kActNone / kActSilu
+};
+struct GnClForward {
+    const void *in;
+    void *out;                       // may be in
+    const float *gamma, *beta;
+    float *mean, *rstd;              // [batch, groups] each, or both null
+    int8_t *codes;                   // checkpoint of `in`, or null
+    uint8_t *scales;
+};
+struct GnClBackward {
+    const void *in;                  // the forward's input, or null: then its checkpoint
+    const int8_t *codes;
+    const uint8_t *scales;
+    const void *grad_out;
+    void *grad_in;                   // may be in or grad_out
+    const float *gamma, *beta, *mean, *rstd;
+    float *grad_gamma, *grad_beta;   // either may be null
+};
+size_t gn_cl_workspace_bytes(const GnClShape &s, bool backward);
+cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void *workspace, cudaStream_t stream);
+cudaError_t gn_cl_backward_launch(const GnClShape &s, const GnClBackward &a, void *workspace, cudaStream_t stream);
+
+// ---- 8-bit activation checkpoints (checkpoint.cu; format in ckpt_device.cuh) ---------------------
+cudaError_t ckpt_pack_launch(const void *src, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim,
+                             int dtype, cudaStream_t stream);
+cudaError_t ckpt_unpack_launch(const int8_t *codes, const uint8_t *scales, void *dst, int64_t rows, int64_t dim,
+                               int dtype, cudaStream_t stream);
+// GEGLU gate [rows, 2 d] -> [rows, d] that also writes the checkpoint of its input.
+cudaError_t geglu_pack_launch(const void *ab, void *dst, int8_t *codes, uint8_t *scales, int64_t rows,
+                              int64_t d, int dtype, cudaStream_t stream);
+// Gradient of the gate's input; the input itself, or its checkpoint when codes != null.
+cudaError_t geglu_backward_launch(const void *ab, const int8_t *codes, const uint8_t *scales, const void *dy,
+                                  void *dab, int64_t rows, int64_t d, int dtype, cudaStream_t stream);
+
 // ---- LayerNorm --------------------------------------------------------------------------------
 cudaError_t ln_launch(const void *in, void *out, const float *w, const float *b, int64_t rows,
                       int64_t dim, float eps, int dtype, cudaStream_t stream);

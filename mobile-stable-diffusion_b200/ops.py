@@ -1,17 +1,18 @@
 """Functional wrappers over the C ABI for torch CUDA tensors.
 
 torch is used for device memory and streams only; every operation below is one call into
-libsdfl.so.  Inputs must be contiguous CUDA tensors of dtype float32 or float16; gamma / beta
-are float32.  Nothing here computes on the host and nothing falls back to torch operators.
+libsdfl.so.  Inputs must be contiguous CUDA tensors of dtype float32 or float16 (the channels-last
+GroupNorm and the checkpoint functions also take bfloat16); gamma / beta are float32.  Nothing here computes on the host and nothing falls back to torch operators.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
 
 from . import _capi
-from ._capi import F16, F32, GN_AUTO, GN_REGISTER, GN_RESIDENT, GN_SPLIT, SdflError, check, lib
+from ._capi import BF16, F16, F32, GN_AUTO, GN_REGISTER, GN_RESIDENT, GN_SPLIT, SdflError, check, lib
 
 __all__ = [
     "groupnorm", "groupnorm_multi", "groupnorm_bias", "chunkwise_add", "groupnorm_noalloc", "groupnorm_plan", "layernorm", "add_layernorm", "gelu_multiply", "silu", "gelu", "quick_gelu",
@@ -19,6 +20,8 @@ __all__ = [
     "local_reduction_variance", "group_norm_apply", "layer_norm_apply", "device_status",
     "selftest_bounded_wait",
     "launch_count", "HostPipeline", "GN_AUTO", "GN_RESIDENT", "GN_SPLIT", "GN_REGISTER", "groupnorm_nhwc", "permute_021", "permute_add", "softmax", "local_softmax", "up_sample_nearest", "concat_channels", "groupnorm_concat",
+    "Checkpoint8", "checkpoint_pack", "checkpoint_unpack", "groupnorm_channels_last", "groupnorm_channels_last_train",
+    "groupnorm_channels_last_backward", "gelu_multiply_checkpoint", "gelu_multiply_backward",
 ]
 
 
@@ -482,6 +485,249 @@ def layer_norm_apply(x, mean, var, weight, bias, chunk_size: int, eps: float = 1
                                   _f32(weight, "weight"), _f32(bias, "bias"), chunk_size,
                                   _dev(out, "out"), x.numel(), eps, _dtype_code(x),
                                   _stream(stream)), "sdfl_layer_norm")
+    return out
+
+
+# ---- channels-last GroupNorm, 8-bit activation checkpoints, gradients --------------------------------
+#
+# These allocate their outputs and workspaces on the stream that the call runs on, so a call inside a
+# graph capture takes them from that graph's pool and shares nothing with another graph.
+
+_TRAIN_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _train_dtype_code(t: torch.Tensor) -> int:
+    code = _TRAIN_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {t.dtype}: float32, float16 or bfloat16 only")
+    return code
+
+
+@contextlib.contextmanager
+def _run_on(device: torch.device, stream):
+    """The device made current, and the stream: work and allocations of the body belong to it."""
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream().cuda_stream
+        else:
+            handle = _stream(stream)
+            s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+            with torch.cuda.stream(s):
+                yield handle
+
+
+def _same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}, not on {t.device}")
+
+
+class Checkpoint8:
+    """An activation kept in 8 bits: `codes` int8 [..., dim] and one scale byte per block of 32 elements
+    of a row, `scales` uint8 [..., ceil(dim / 32)]; an element stands for code * 2^(scale - 127).
+    `dtype` is the type of the tensor it was made from (and of its expansion)."""
+
+    __slots__ = ("codes", "scales", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype):
+        if dtype not in _TRAIN_DTYPES:
+            raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16 only")
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise TypeError("codes must be int8 and scales uint8")
+        if codes.dim() < 1 or scales.shape != codes.shape[:-1] + (-(-codes.shape[-1] // 32),):
+            raise ValueError("scales must be [..., ceil(dim / 32)] for codes [..., dim]")
+        self.codes, self.scales, self.dtype = codes, scales, dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _empty_checkpoint(x: torch.Tensor) -> Checkpoint8:
+    shape = tuple(x.shape)
+    return Checkpoint8(torch.empty(shape, dtype=torch.int8, device=x.device),
+                       torch.empty(shape[:-1] + (-(-shape[-1] // 32),), dtype=torch.uint8, device=x.device), x.dtype)
+
+
+def _rows(x) -> tuple[int, int]:
+    dim = x.shape[-1]
+    rows = 1
+    for n in x.shape[:-1]:
+        rows *= n
+    return rows, dim
+
+
+def checkpoint_pack(x: torch.Tensor, stream=None) -> Checkpoint8:
+    """A checkpoint of x [..., dim] in 8 bits per element (format: sdfl_checkpoint_pack)."""
+    code = _train_dtype_code(x)
+    _dev(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    rows, dim = _rows(x)
+    with _run_on(x.device, stream) as s:
+        kept = _empty_checkpoint(x)
+        check(lib.sdfl_checkpoint_pack(x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), rows, dim, code, s),
+              "sdfl_checkpoint_pack")
+    return kept
+
+
+def checkpoint_unpack(kept: Checkpoint8, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The values of a checkpoint, in its dtype (or in out's: every value is exact in all three)."""
+    _dev(kept.codes, "codes"), _dev(kept.scales, "scales")
+    rows, dim = _rows(kept)
+    with _run_on(kept.device, stream) as s:
+        out = torch.empty(kept.shape, dtype=kept.dtype, device=kept.device) if out is None else out
+        if out.shape != kept.shape:
+            raise ValueError("out must have the checkpoint's shape")
+        _same_device(kept.device, scales=kept.scales, out=out)
+        check(lib.sdfl_checkpoint_unpack(kept.codes.data_ptr(), kept.scales.data_ptr(), _dev(out, "out"), rows, dim,
+                                         _train_dtype_code(out), s), "sdfl_checkpoint_unpack")
+    return out
+
+
+def _gn_cl_shape(x) -> tuple[int, int, int]:
+    if len(x.shape) < 2:
+        raise ValueError("x must be [batch, ..., channels]")
+    B, Cc = x.shape[0], x.shape[-1]
+    hw = 1
+    for n in x.shape[1:-1]:
+        hw *= n
+    return B, Cc, hw
+
+
+def _gn_cl_forward(x, gamma, beta, num_groups, eps, silu, out, stream, stats, checkpoint):
+    code = _train_dtype_code(x)
+    _dev(x, "x")
+    B, Cc, hw = _gn_cl_shape(x)
+    if gamma.numel() != Cc or beta.numel() != Cc:
+        raise ValueError("gamma and beta must have one entry per channel")
+    _same_device(x.device, gamma=gamma, beta=beta, out=out)
+    mean = rstd = kept = None
+    with _run_on(x.device, stream) as s:
+        out = torch.empty_like(x) if out is None else out
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must match x in shape and dtype")
+        if stats:
+            make = torch.empty if x.numel() else torch.zeros
+            mean = make((B, num_groups), dtype=torch.float32, device=x.device)
+            rstd = make((B, num_groups), dtype=torch.float32, device=x.device)
+        if checkpoint:
+            kept = _empty_checkpoint(x)
+        nbytes = lib.sdfl_groupnorm_channels_last_workspace_bytes(B, Cc, hw, num_groups, 0, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        check(lib.sdfl_groupnorm_channels_last_forward(
+            x.data_ptr(), _dev(out, "out"), _f32(gamma, "gamma"), _f32(beta, "beta"),
+            mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
+            kept.codes.data_ptr() if checkpoint else None, kept.scales.data_ptr() if checkpoint else None,
+            B, Cc, hw, num_groups, eps, int(silu), code, ws.data_ptr() if nbytes else None, nbytes, s),
+            "sdfl_groupnorm_channels_last_forward")
+    return out, mean, rstd, kept
+
+
+def groupnorm_channels_last(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, num_groups: int,
+                            eps: float = 1e-5, silu: bool = False, out: torch.Tensor | None = None,
+                            stream=None) -> torch.Tensor:
+    """GroupNorm(+SiLU) of a channels-last tensor [B, ..., C]; out may be x itself.  A torch tensor in
+    channels_last memory format is that after x.permute(0, 2, 3, 1)."""
+    return _gn_cl_forward(x, gamma, beta, num_groups, eps, silu, out, stream, False, False)[0]
+
+
+def groupnorm_channels_last_train(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, num_groups: int,
+                                  eps: float = 1e-5, silu: bool = False, checkpoint: bool = False,
+                                  out: torch.Tensor | None = None, stream=None):
+    """The forward pass of a training step: (y, mean, rstd, source), where source is what
+    groupnorm_channels_last_backward will read: x itself, or with checkpoint=True a Checkpoint8 of x
+    written in the same pass, after which x may be dropped or (out=x) overwritten.
+    Without a checkpoint, out=x would destroy what the backward pass needs and is refused."""
+    if not checkpoint and out is not None and x.numel() and out.data_ptr() == x.data_ptr():
+        raise ValueError("out=x needs checkpoint=True: the backward pass reads x")
+    y, mean, rstd, kept = _gn_cl_forward(x, gamma, beta, num_groups, eps, silu, out, stream, True, checkpoint)
+    return y, mean, rstd, kept if checkpoint else x
+
+
+def groupnorm_channels_last_backward(grad_out: torch.Tensor, source, mean: torch.Tensor, rstd: torch.Tensor,
+                                     gamma: torch.Tensor, beta: torch.Tensor, num_groups: int, silu: bool = False,
+                                     out: torch.Tensor | None = None, stream=None):
+    """(grad_x, grad_gamma, grad_beta) from the forward's input or its Checkpoint8 and the saved
+    statistics.  out (for grad_x) may be grad_out or, when it is a tensor, source."""
+    code = _train_dtype_code(grad_out)
+    _dev(grad_out, "grad_out")
+    if source.shape != grad_out.shape or source.dtype != grad_out.dtype:
+        raise ValueError("source must match grad_out in shape and dtype")
+    B, Cc, hw = _gn_cl_shape(grad_out)
+    if gamma.numel() != Cc or beta.numel() != Cc:
+        raise ValueError("gamma and beta must have one entry per channel")
+    if mean.shape != (B, num_groups) or rstd.shape != (B, num_groups):
+        raise ValueError("mean and rstd must be [batch, num_groups]")
+    kept = isinstance(source, Checkpoint8)
+    device = grad_out.device
+    _same_device(device, source=source.codes if kept else source, scales=source.scales if kept else None, mean=mean,
+                 rstd=rstd, gamma=gamma, beta=beta, out=out)
+    with _run_on(device, stream) as s:
+        out = torch.empty_like(grad_out) if out is None else out
+        if out.shape != grad_out.shape or out.dtype != grad_out.dtype:
+            raise ValueError("out must match grad_out in shape and dtype")
+        grad_gamma = torch.empty(Cc, dtype=torch.float32, device=device)
+        grad_beta = torch.empty(Cc, dtype=torch.float32, device=device)
+        nbytes = lib.sdfl_groupnorm_channels_last_workspace_bytes(B, Cc, hw, num_groups, 1, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        check(lib.sdfl_groupnorm_channels_last_backward(
+            None if kept else _dev(source, "source"), _dev(source.codes, "codes") if kept else None,
+            _dev(source.scales, "scales") if kept else None, grad_out.data_ptr(), _dev(out, "out"),
+            _f32(gamma, "gamma"), _f32(beta, "beta"), _f32(mean, "mean"), _f32(rstd, "rstd"), grad_gamma.data_ptr(),
+            grad_beta.data_ptr(), B, Cc, hw, num_groups, int(silu), code, ws.data_ptr() if nbytes else None, nbytes, s),
+            "sdfl_groupnorm_channels_last_backward")
+    return out, grad_gamma, grad_beta
+
+
+def gelu_multiply_checkpoint(ab: torch.Tensor, out: torch.Tensor | None = None, stream=None):
+    """(gelu_multiply(ab), Checkpoint8 of ab): the forward pass of a training step, ab not needed after it."""
+    code = _train_dtype_code(ab)
+    _dev(ab, "ab")
+    if ab.dim() < 1 or ab.shape[-1] % 2:
+        raise ValueError("last dimension must be even")
+    rows, dim = _rows(ab)
+    with _run_on(ab.device, stream) as s:
+        shape = tuple(ab.shape[:-1]) + (dim // 2,)
+        out = torch.empty(shape, dtype=ab.dtype, device=ab.device) if out is None else out
+        if tuple(out.shape) != shape or out.dtype != ab.dtype:
+            raise ValueError("out must be [..., dim / 2] of ab's dtype")
+        _same_device(ab.device, out=out)
+        kept = _empty_checkpoint(ab)
+        check(lib.sdfl_gelu_multiply_checkpoint(ab.data_ptr(), _dev(out, "out"), kept.codes.data_ptr(),
+                                                kept.scales.data_ptr(), rows, dim // 2, code, s),
+              "sdfl_gelu_multiply_checkpoint")
+    return out, kept
+
+
+def gelu_multiply_backward(grad_out: torch.Tensor, source, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Gradient of gelu_multiply's input [..., 2D] from grad_out [..., D] and that input or its
+    Checkpoint8.  out may be the input itself."""
+    code = _train_dtype_code(grad_out)
+    _dev(grad_out, "grad_out")
+    if grad_out.dim() < 1 or tuple(source.shape) != tuple(grad_out.shape[:-1]) + (2 * grad_out.shape[-1],) \
+            or source.dtype != grad_out.dtype:
+        raise ValueError("source must be [..., 2D] of grad_out's dtype for grad_out [..., D]")
+    rows, dim = _rows(grad_out)
+    kept = isinstance(source, Checkpoint8)
+    device = grad_out.device
+    _same_device(device, source=source.codes if kept else source, scales=source.scales if kept else None, out=out)
+    with _run_on(device, stream) as s:
+        out = torch.empty(source.shape, dtype=grad_out.dtype, device=device) if out is None else out
+        if out.shape != source.shape or out.dtype != grad_out.dtype:
+            raise ValueError("out must match source in shape and dtype")
+        check(lib.sdfl_gelu_multiply_backward(
+            None if kept else _dev(source, "source"), _dev(source.codes, "codes") if kept else None,
+            _dev(source.scales, "scales") if kept else None, grad_out.data_ptr(), _dev(out, "out"), rows, dim, code, s),
+            "sdfl_gelu_multiply_backward")
     return out
 
 
