@@ -6,8 +6,8 @@ GroupNorm and the checkpoint functions also take bfloat16); gamma / beta are flo
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -503,23 +503,38 @@ def _train_dtype_code(t: torch.Tensor) -> int:
     return code
 
 
-@contextlib.contextmanager
-def _run_on(device: torch.device, stream):
-    """The device made current, and the stream: work and allocations of the body belong to it."""
-    with torch.cuda.device(device):
-        if stream is None:
-            yield torch.cuda.current_stream().cuda_stream
-        else:
-            handle = _stream(stream)
-            s = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-            with torch.cuda.stream(s):
-                yield handle
+# The current stream's handle without building a torch.cuda.Stream object (2 us of a 10 us call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, not on {t.device}")
+def _run_on(index: int, stream, body):
+    """body(stream handle) with device `index` current and, if a stream is given, that stream: its
+    work and its allocations belong to it."""
+    if stream is None:
+        if index == torch.cuda.current_device():
+            return body(_raw_stream(index))
+        with torch.cuda.device(index):
+            return body(_raw_stream(index))
+    handle = _stream(stream)
+    with torch.cuda.device(index):
+        s = torch.cuda.ExternalStream(handle, device=index) if handle else torch.cuda.default_stream(index)
+        with torch.cuda.stream(s):
+            return body(handle)
+
+
+def _on(index: int, t: torch.Tensor, name: str) -> int:
+    """Address of a contiguous tensor on CUDA device `index`."""
+    p = _dev(t, name)
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}, not on {t.device}")
+    return p
+
+
+def _f32_on(index: int, t: torch.Tensor, name: str) -> int:
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32")
+    return _on(index, t, name)
 
 
 class Checkpoint8:
@@ -534,7 +549,8 @@ class Checkpoint8:
             raise TypeError(f"unsupported dtype {dtype}: float32, float16 or bfloat16 only")
         if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
             raise TypeError("codes must be int8 and scales uint8")
-        if codes.dim() < 1 or scales.shape != codes.shape[:-1] + (-(-codes.shape[-1] // 32),):
+        shape = codes.shape
+        if not shape or scales.shape != shape[:-1] + (-(-shape[-1] // 32),):
             raise ValueError("scales must be [..., ceil(dim / 32)] for codes [..., dim]")
         self.codes, self.scales, self.dtype = codes, scales, dtype
 
@@ -552,51 +568,68 @@ class Checkpoint8:
 
 
 def _empty_checkpoint(x: torch.Tensor) -> Checkpoint8:
-    shape = tuple(x.shape)
-    return Checkpoint8(torch.empty(shape, dtype=torch.int8, device=x.device),
-                       torch.empty(shape[:-1] + (-(-shape[-1] // 32),), dtype=torch.uint8, device=x.device), x.dtype)
+    shape = x.shape
+    return Checkpoint8(torch.empty_like(x, dtype=torch.int8),
+                       x.new_empty(shape[:-1] + (-(-shape[-1] // 32),), dtype=torch.uint8), x.dtype)
 
 
-def _rows(x) -> tuple[int, int]:
-    dim = x.shape[-1]
-    rows = 1
-    for n in x.shape[:-1]:
-        rows *= n
-    return rows, dim
+def _source_on(index: int, source) -> tuple:
+    """(tensor, codes, scales) addresses of a backward pass's source."""
+    if isinstance(source, Checkpoint8):
+        return None, _on(index, source.codes, "codes"), _on(index, source.scales, "scales")
+    return _on(index, source, "source"), None, None
 
 
 def checkpoint_pack(x: torch.Tensor, stream=None) -> Checkpoint8:
     """A checkpoint of x [..., dim] in 8 bits per element (format: sdfl_checkpoint_pack)."""
     code = _train_dtype_code(x)
-    _dev(x, "x")
+    p = _dev(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
-    rows, dim = _rows(x)
-    with _run_on(x.device, stream) as s:
+    dim = x.shape[-1]
+    rows = x.numel() // dim if dim else 0
+
+    def body(s):
         kept = _empty_checkpoint(x)
-        check(lib.sdfl_checkpoint_pack(x.data_ptr(), kept.codes.data_ptr(), kept.scales.data_ptr(), rows, dim, code, s),
+        check(lib.sdfl_checkpoint_pack(p, kept.codes.data_ptr(), kept.scales.data_ptr(), rows, dim, code, s),
               "sdfl_checkpoint_pack")
-    return kept
+        return kept
+    return _run_on(x.get_device(), stream, body)
 
 
 def checkpoint_unpack(kept: Checkpoint8, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-    """The values of a checkpoint, in its dtype (or in out's: every value is exact in all three)."""
-    _dev(kept.codes, "codes"), _dev(kept.scales, "scales")
-    rows, dim = _rows(kept)
-    with _run_on(kept.device, stream) as s:
-        out = torch.empty(kept.shape, dtype=kept.dtype, device=kept.device) if out is None else out
-        if out.shape != kept.shape:
+    """The values of a checkpoint, in its dtype, or in out's (a value is exact in all three types, unless
+    it lies outside a narrower type's range)."""
+    codes = _dev(kept.codes, "codes")
+    index = kept.codes.get_device()
+    scales = _on(index, kept.scales, "scales")
+    dim = kept.shape[-1]
+    rows = kept.codes.numel() // dim if dim else 0
+
+    def body(s):
+        y = torch.empty_like(kept.codes, dtype=kept.dtype) if out is None else out
+        if y.shape != kept.shape:
             raise ValueError("out must have the checkpoint's shape")
-        _same_device(kept.device, scales=kept.scales, out=out)
-        check(lib.sdfl_checkpoint_unpack(kept.codes.data_ptr(), kept.scales.data_ptr(), _dev(out, "out"), rows, dim,
-                                         _train_dtype_code(out), s), "sdfl_checkpoint_unpack")
-    return out
+        check(lib.sdfl_checkpoint_unpack(codes, scales, _on(index, y, "out"), rows, dim, _train_dtype_code(y), s),
+              "sdfl_checkpoint_unpack")
+        return y
+    return _run_on(index, stream, body)
 
 
-def _gn_cl_shape(x) -> tuple[int, int, int]:
-    if len(x.shape) < 2:
+@functools.lru_cache(maxsize=1024)
+def _gn_cl_workspace_bytes(index, B, Cc, hw, num_groups, backward, code) -> int:
+    # `index` is the current device: the plan, and with it the answer, goes by its number of SMs
+    return lib.sdfl_groupnorm_channels_last_workspace_bytes(B, Cc, hw, num_groups, backward, code)
+
+
+def _gn_cl_shape(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor) -> tuple[int, int, int]:
+    if x.dim() < 2:
         raise ValueError("x must be [batch, ..., channels]")
     B, Cc = x.shape[0], x.shape[-1]
+    if gamma.numel() != Cc or beta.numel() != Cc:
+        raise ValueError("gamma and beta must have one entry per channel")
+    if B * Cc:
+        return B, Cc, x.numel() // (B * Cc)
     hw = 1
     for n in x.shape[1:-1]:
         hw *= n
@@ -605,31 +638,33 @@ def _gn_cl_shape(x) -> tuple[int, int, int]:
 
 def _gn_cl_forward(x, gamma, beta, num_groups, eps, silu, out, stream, stats, checkpoint):
     code = _train_dtype_code(x)
-    _dev(x, "x")
-    B, Cc, hw = _gn_cl_shape(x)
-    if gamma.numel() != Cc or beta.numel() != Cc:
-        raise ValueError("gamma and beta must have one entry per channel")
-    _same_device(x.device, gamma=gamma, beta=beta, out=out)
-    mean = rstd = kept = None
-    with _run_on(x.device, stream) as s:
-        out = torch.empty_like(x) if out is None else out
-        if out.shape != x.shape or out.dtype != x.dtype:
+    p = _dev(x, "x")
+    index = x.get_device()
+    B, Cc, hw = _gn_cl_shape(x, gamma, beta)
+    g, b = _f32_on(index, gamma, "gamma"), _f32_on(index, beta, "beta")
+
+    def body(s):
+        y = torch.empty_like(x) if out is None else out
+        if y.shape != x.shape or y.dtype != x.dtype:
             raise ValueError("out must match x in shape and dtype")
+        mean = rstd = kept = pm = pr = pc = ps = pw = None
         if stats:
-            make = torch.empty if x.numel() else torch.zeros
-            mean = make((B, num_groups), dtype=torch.float32, device=x.device)
-            rstd = make((B, num_groups), dtype=torch.float32, device=x.device)
+            make = x.new_empty if x.numel() else x.new_zeros
+            mean = make((B, num_groups), dtype=torch.float32)
+            rstd = make((B, num_groups), dtype=torch.float32)
+            pm, pr = mean.data_ptr(), rstd.data_ptr()
         if checkpoint:
             kept = _empty_checkpoint(x)
-        nbytes = lib.sdfl_groupnorm_channels_last_workspace_bytes(B, Cc, hw, num_groups, 0, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        check(lib.sdfl_groupnorm_channels_last_forward(
-            x.data_ptr(), _dev(out, "out"), _f32(gamma, "gamma"), _f32(beta, "beta"),
-            mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
-            kept.codes.data_ptr() if checkpoint else None, kept.scales.data_ptr() if checkpoint else None,
-            B, Cc, hw, num_groups, eps, int(silu), code, ws.data_ptr() if nbytes else None, nbytes, s),
-            "sdfl_groupnorm_channels_last_forward")
-    return out, mean, rstd, kept
+            pc, ps = kept.codes.data_ptr(), kept.scales.data_ptr()
+        nbytes = _gn_cl_workspace_bytes(index, B, Cc, hw, num_groups, 0, code)
+        if nbytes:
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            pw = ws.data_ptr()
+        check(lib.sdfl_groupnorm_channels_last_forward(p, _on(index, y, "out"), g, b, pm, pr, pc, ps, B, Cc, hw, num_groups,
+                                                       eps, int(silu), code, pw, nbytes, s),
+              "sdfl_groupnorm_channels_last_forward")
+        return y, mean, rstd, kept
+    return _run_on(index, stream, body)
 
 
 def groupnorm_channels_last(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, num_groups: int,
@@ -645,7 +680,7 @@ def groupnorm_channels_last_train(x: torch.Tensor, gamma: torch.Tensor, beta: to
                                   out: torch.Tensor | None = None, stream=None):
     """The forward pass of a training step: (y, mean, rstd, source), where source is what
     groupnorm_channels_last_backward will read: x itself, or with checkpoint=True a Checkpoint8 of x
-    written in the same pass, after which x may be dropped or (out=x) overwritten.
+    written in the same call, after which x may be dropped or (out=x) overwritten.
     Without a checkpoint, out=x would destroy what the backward pass needs and is refused."""
     if not checkpoint and out is not None and x.numel() and out.data_ptr() == x.data_ptr():
         raise ValueError("out=x needs checkpoint=True: the backward pass reads x")
@@ -659,76 +694,79 @@ def groupnorm_channels_last_backward(grad_out: torch.Tensor, source, mean: torch
     """(grad_x, grad_gamma, grad_beta) from the forward's input or its Checkpoint8 and the saved
     statistics.  out (for grad_x) may be grad_out or, when it is a tensor, source."""
     code = _train_dtype_code(grad_out)
-    _dev(grad_out, "grad_out")
+    d = _dev(grad_out, "grad_out")
+    index = grad_out.get_device()
     if source.shape != grad_out.shape or source.dtype != grad_out.dtype:
         raise ValueError("source must match grad_out in shape and dtype")
-    B, Cc, hw = _gn_cl_shape(grad_out)
-    if gamma.numel() != Cc or beta.numel() != Cc:
-        raise ValueError("gamma and beta must have one entry per channel")
+    B, Cc, hw = _gn_cl_shape(grad_out, gamma, beta)
     if mean.shape != (B, num_groups) or rstd.shape != (B, num_groups):
         raise ValueError("mean and rstd must be [batch, num_groups]")
-    kept = isinstance(source, Checkpoint8)
-    device = grad_out.device
-    _same_device(device, source=source.codes if kept else source, scales=source.scales if kept else None, mean=mean,
-                 rstd=rstd, gamma=gamma, beta=beta, out=out)
-    with _run_on(device, stream) as s:
-        out = torch.empty_like(grad_out) if out is None else out
-        if out.shape != grad_out.shape or out.dtype != grad_out.dtype:
+    x, codes, scales = _source_on(index, source)
+    g, b = _f32_on(index, gamma, "gamma"), _f32_on(index, beta, "beta")
+    m, r = _f32_on(index, mean, "mean"), _f32_on(index, rstd, "rstd")
+
+    def body(s):
+        dx = torch.empty_like(grad_out) if out is None else out
+        if dx.shape != grad_out.shape or dx.dtype != grad_out.dtype:
             raise ValueError("out must match grad_out in shape and dtype")
-        grad_gamma = torch.empty(Cc, dtype=torch.float32, device=device)
-        grad_beta = torch.empty(Cc, dtype=torch.float32, device=device)
-        nbytes = lib.sdfl_groupnorm_channels_last_workspace_bytes(B, Cc, hw, num_groups, 1, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        check(lib.sdfl_groupnorm_channels_last_backward(
-            None if kept else _dev(source, "source"), _dev(source.codes, "codes") if kept else None,
-            _dev(source.scales, "scales") if kept else None, grad_out.data_ptr(), _dev(out, "out"),
-            _f32(gamma, "gamma"), _f32(beta, "beta"), _f32(mean, "mean"), _f32(rstd, "rstd"), grad_gamma.data_ptr(),
-            grad_beta.data_ptr(), B, Cc, hw, num_groups, int(silu), code, ws.data_ptr() if nbytes else None, nbytes, s),
-            "sdfl_groupnorm_channels_last_backward")
-    return out, grad_gamma, grad_beta
+        grad_gamma = grad_out.new_empty(Cc, dtype=torch.float32)
+        grad_beta = grad_out.new_empty(Cc, dtype=torch.float32)
+        nbytes = _gn_cl_workspace_bytes(index, B, Cc, hw, num_groups, 1, code)
+        pw = None
+        if nbytes:
+            ws = grad_out.new_empty(nbytes, dtype=torch.uint8)
+            pw = ws.data_ptr()
+        check(lib.sdfl_groupnorm_channels_last_backward(x, codes, scales, d, _on(index, dx, "out"), g, b, m, r,
+                                                        grad_gamma.data_ptr(), grad_beta.data_ptr(), B, Cc, hw, num_groups,
+                                                        int(silu), code, pw, nbytes, s),
+              "sdfl_groupnorm_channels_last_backward")
+        return dx, grad_gamma, grad_beta
+    return _run_on(index, stream, body)
 
 
 def gelu_multiply_checkpoint(ab: torch.Tensor, out: torch.Tensor | None = None, stream=None):
     """(gelu_multiply(ab), Checkpoint8 of ab): the forward pass of a training step, ab not needed after it."""
     code = _train_dtype_code(ab)
-    _dev(ab, "ab")
+    p = _dev(ab, "ab")
+    index = ab.get_device()
     if ab.dim() < 1 or ab.shape[-1] % 2:
         raise ValueError("last dimension must be even")
-    rows, dim = _rows(ab)
-    with _run_on(ab.device, stream) as s:
-        shape = tuple(ab.shape[:-1]) + (dim // 2,)
-        out = torch.empty(shape, dtype=ab.dtype, device=ab.device) if out is None else out
-        if tuple(out.shape) != shape or out.dtype != ab.dtype:
+    D = ab.shape[-1] // 2
+    rows = ab.numel() // (2 * D) if D else 0
+    shape = ab.shape[:-1] + (D,)
+
+    def body(s):
+        y = ab.new_empty(shape) if out is None else out
+        if y.shape != shape or y.dtype != ab.dtype:
             raise ValueError("out must be [..., dim / 2] of ab's dtype")
-        _same_device(ab.device, out=out)
         kept = _empty_checkpoint(ab)
-        check(lib.sdfl_gelu_multiply_checkpoint(ab.data_ptr(), _dev(out, "out"), kept.codes.data_ptr(),
-                                                kept.scales.data_ptr(), rows, dim // 2, code, s),
-              "sdfl_gelu_multiply_checkpoint")
-    return out, kept
+        check(lib.sdfl_gelu_multiply_checkpoint(p, _on(index, y, "out"), kept.codes.data_ptr(), kept.scales.data_ptr(), rows,
+                                                D, code, s), "sdfl_gelu_multiply_checkpoint")
+        return y, kept
+    return _run_on(index, stream, body)
 
 
 def gelu_multiply_backward(grad_out: torch.Tensor, source, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Gradient of gelu_multiply's input [..., 2D] from grad_out [..., D] and that input or its
     Checkpoint8.  out may be the input itself."""
     code = _train_dtype_code(grad_out)
-    _dev(grad_out, "grad_out")
-    if grad_out.dim() < 1 or tuple(source.shape) != tuple(grad_out.shape[:-1]) + (2 * grad_out.shape[-1],) \
-            or source.dtype != grad_out.dtype:
+    d = _dev(grad_out, "grad_out")
+    index = grad_out.get_device()
+    shape = source.shape
+    if grad_out.dim() < 1 or shape != grad_out.shape[:-1] + (2 * grad_out.shape[-1],) or source.dtype != grad_out.dtype:
         raise ValueError("source must be [..., 2D] of grad_out's dtype for grad_out [..., D]")
-    rows, dim = _rows(grad_out)
-    kept = isinstance(source, Checkpoint8)
-    device = grad_out.device
-    _same_device(device, source=source.codes if kept else source, scales=source.scales if kept else None, out=out)
-    with _run_on(device, stream) as s:
-        out = torch.empty(source.shape, dtype=grad_out.dtype, device=device) if out is None else out
-        if out.shape != source.shape or out.dtype != grad_out.dtype:
+    D = grad_out.shape[-1]
+    rows = grad_out.numel() // D if D else 0
+    ab, codes, scales = _source_on(index, source)
+
+    def body(s):
+        dab = grad_out.new_empty(shape) if out is None else out
+        if dab.shape != shape or dab.dtype != grad_out.dtype:
             raise ValueError("out must match source in shape and dtype")
-        check(lib.sdfl_gelu_multiply_backward(
-            None if kept else _dev(source, "source"), _dev(source.codes, "codes") if kept else None,
-            _dev(source.scales, "scales") if kept else None, grad_out.data_ptr(), _dev(out, "out"), rows, dim, code, s),
-            "sdfl_gelu_multiply_backward")
-    return out
+        check(lib.sdfl_gelu_multiply_backward(ab, codes, scales, d, _on(index, dab, "out"), rows, D, code, s),
+              "sdfl_gelu_multiply_backward")
+        return dab
+    return _run_on(index, stream, body)
 
 
 class HostPipeline:

@@ -65,7 +65,7 @@ def test_forward_and_backward(sdfl, B, P, C, G, dtype):
     assert_within(mean, wmean, K * U * size + 1e-30, "mean")
     # the variance's own roundings, and the mean's error squared against it
     assert_within(rstd, wrstd, wrstd * (K * U + (K * U * size * wrstd) ** 2), "rstd")
-    assert torch.equal(ops.groupnorm_channels_last(dx_, dg, db, G, EPS, silu), y)
+    check_forward(ops.groupnorm_channels_last(dx_, dg, db, G, EPS, silu), x, gamma, beta, G, silu, dtype, "inference")
     codes, scales, values = checkpoint_reference(x)
     assert torch.equal(kept.codes.cpu(), codes) and torch.equal(kept.scales.cpu(), scales)
 

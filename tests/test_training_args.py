@@ -127,7 +127,6 @@ def test_python_refusals_on_the_device():
     st = torch.ones((2, 8), device="cuda")
     for call in (lambda: ops.groupnorm_channels_last(x.transpose(1, 2), w, w, 8),
                  lambda: ops.groupnorm_channels_last(x, w2, w, 8),
-                 lambda: ops.groupnorm_channels_last(x, w.cpu(), w, 8),
                  lambda: ops.groupnorm_channels_last(x, w, w, 8, out=torch.empty_like(x, dtype=torch.float32)),
                  lambda: ops.groupnorm_channels_last_train(x, w, w, 8, out=x),
                  lambda: ops.groupnorm_channels_last_backward(x, kept, st[:1], st, w, w, 8),
@@ -142,3 +141,5 @@ def test_python_refusals_on_the_device():
         ops.groupnorm_channels_last(x, w, w, 7)
     with pytest.raises(TypeError):
         ops.groupnorm_channels_last(x, w.half(), w, 8)
+    with pytest.raises(TypeError):
+        ops.groupnorm_channels_last(x, w.cpu(), w, 8)
