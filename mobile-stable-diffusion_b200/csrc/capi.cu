@@ -693,11 +693,12 @@ int sdfl_gelu_multiply_backward(const void *AB, const int8_t *codes, const uint8
 
 int sdfl_device_status(unsigned int *value, int clear, void *stream) {
     if (!value) return SDFL_ERR_INVALID_POINTER;
-    unsigned int ring = 0, multi = 0, reg = 0;
+    unsigned int ring = 0, multi = 0, reg = 0, cl = 0;
     cudaError_t e = sdfl::gn_read_status(&ring, clear != 0, as_stream(stream));
     if (e == cudaSuccess) e = sdfl::gn_multi_read_status(&multi, clear != 0, as_stream(stream));
     if (e == cudaSuccess) e = sdfl::gn_register_read_status(&reg, clear != 0, as_stream(stream));
-    *value = ring | multi | reg;
+    if (e == cudaSuccess) e = sdfl::gn_cl_read_status(&cl, clear != 0, as_stream(stream));
+    *value = ring | multi | reg | cl;
     return wrap(e);
 }
 

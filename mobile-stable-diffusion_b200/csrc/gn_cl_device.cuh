@@ -80,92 +80,108 @@ template <typename T> struct Source<T, 1, true> {
     __device__ __forceinline__ void values(float (&f)[1]) const { f[0] = ckpt_value(c, e); }
 };
 
-// ---- sums over the rows of a thread block ----------------------------------------------------------
-// buf[row * ncols + c] summed over `rows` rows into buf[c], pairwise (error of log2(rows) roundings,
-// and the same order on every run).  Synchronises before and after.
-__device__ __forceinline__ void fold_rows(float *buf, int rows, int ncols) {
-    __syncthreads();
-    while (rows > 1) {
-        const int half = (rows + 1) >> 1;
-        const int n = (rows - half) * ncols;
-        for (int i = threadIdx.x; i < n; i += blockDim.x) buf[i] += buf[i + half * ncols];
-        rows = half;
-        __syncthreads();
-    }
-}
+// ---- arithmetic on a column: VEC elements as VEC / 2 pairs ------------------------------------------
+// The packed fp32 instructions (add, mul and fma .f32x2) do two elements per issue slot, and issue slots
+// are what these kernels run short of next to HBM.  VEC = 1 uses the scalar forms.
+using Pair = unsigned long long;
 
-// ---- running moments of a thread's column: shifted sums around the first value seen ----------------
-template <int VEC> struct ColumnMoments {
-    float k[VEC], s[VEC], q[VEC];
-    __device__ __forceinline__ void first(const float (&f)[VEC]) {
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(Pair p, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair vadd(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair vmul(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair vfma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+
+template <int VEC> struct Column {
+    using E = Pair;
+    static constexpr int N = VEC / 2;
+    Pair e[N];
+    static __device__ __forceinline__ Pair all(float x) { return pair(x, x); }
+    __device__ __forceinline__ void set(const float *f) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { k[i] = f[i]; s[i] = 0.f; q[i] = 0.f; }
+        for (int i = 0; i < N; ++i) e[i] = pair(f[2 * i], f[2 * i + 1]);
     }
-    __device__ __forceinline__ void add(const float (&f)[VEC]) {
+    __device__ __forceinline__ void get(float *f) const {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float d = f[i] - k[i];
-            s[i] += d;
-            q[i] = fmaf(d, d, q[i]);
-        }
+        for (int i = 0; i < N; ++i) split(e[i], f[2 * i], f[2 * i + 1]);
     }
 };
-
-// Moments of every column's channels over the block's rows: mean[c] and m2[c] (squared deviations from
-// that mean), c < ncols, out of each thread's n values per channel.  First the means, then the
-// deviations from them as M2_thread + n (mean_thread - mean)^2: only non-negative terms, nothing
-// cancels.  buf: threads * VEC floats, mean: ncols floats; m2 comes back in buf.
-template <int VEC>
-__device__ __forceinline__ void block_moments(const ColumnMoments<VEC> &m, float n, bool active, int row, int rows,
-                                              int col, int ncols, float count, float *buf, float *mean) {
-    __syncthreads();                 // the buffers may still be read from the call before
-    const float inv = n > 0.f ? 1.0f / n : 0.f;
-    float *mine = buf + row * ncols + col * VEC;
-    if (active) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) mine[i] = n > 0.f ? fmaf(n, m.k[i], m.s[i]) : 0.f;
-    }
-    fold_rows(buf, rows, ncols);
-    for (int c = threadIdx.x; c < ncols; c += blockDim.x) mean[c] = buf[c] / count;
-    __syncthreads();
-    if (active) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float t = m.s[i] * inv;
-            const float d = m.k[i] + t - mean[col * VEC + i];
-            mine[i] = n > 0.f ? fmaxf(fmaf(-m.s[i], t, m.q[i]), 0.f) + n * d * d : 0.f;
-        }
-    }
-    fold_rows(buf, rows, ncols);
-}
-
-// ---- per-channel arithmetic ------------------------------------------------------------------------
-// 1 / (1 + exp(-z)) with the SFU exp2 and reciprocal (relative error about 2^-22 each).
-__device__ __forceinline__ float sigmoid_fast(float z) { return rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z)); }
-
-// fp32 storage keeps (x - mean) as its own step; half storage folds the affine into one multiply-add
-// (the folded constant's rounding, 2^-24 |mean| rstd, is far below half a step of the output).
-template <typename T, int VEC, int ACT> struct Normalise {
-    float p[VEC], q[VEC], r[VEC];       // half: z = x p + q;  fp32: z = (x - r) p + q
-    __device__ __forceinline__ void set(int i, float mean, float rstd, float w, float b) {
-        p[i] = w * rstd;
-        if (sizeof(T) == 2) { q[i] = fmaf(-mean, p[i], b); r[i] = 0.f; }
-        else { q[i] = b; r[i] = mean; }
-    }
-    __device__ __forceinline__ void apply(float (&f)[VEC]) const {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float z = sizeof(T) == 2 ? fmaf(f[i], p[i], q[i]) : fmaf(f[i] - r[i], p[i], q[i]);
-            f[i] = ACT == kActSilu ? z * sigmoid_fast(z) : z;
-        }
-    }
+template <> struct Column<1> {
+    using E = float;
+    static constexpr int N = 1;
+    float e[1];
+    static __device__ __forceinline__ float all(float x) { return x; }
+    __device__ __forceinline__ void set(const float *f) { e[0] = f[0]; }
+    __device__ __forceinline__ void get(float *f) const { f[0] = e[0]; }
 };
 
-// dz = dy act'(z), silu'(z) = s + z s (1 - s) with s = sigmoid(z).
-template <int ACT> __device__ __forceinline__ float act_grad(float dy, float z) {
+// VEC floats of shared memory, 16 bytes at a time (rows of a thread's column are 16-byte aligned).
+template <int VEC> __device__ __forceinline__ void shared_store(float *to, const float (&f)[VEC]) {
+    if constexpr (VEC == 1) to[0] = f[0];
+    else
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4)
+            *reinterpret_cast<float4 *>(to + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+}
+template <int VEC> __device__ __forceinline__ void shared_load(const float *from, float (&f)[VEC]) {
+    if constexpr (VEC == 1) f[0] = from[0];
+    else
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(from + i);
+            f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+        }
+}
+
+template <int VEC> __device__ __forceinline__ void column_load(const float *from, Column<VEC> &c) {
+    float f[VEC];
+    shared_load<VEC>(from, f);
+    c.set(f);
+}
+template <int VEC> __device__ __forceinline__ void column_store(float *to, const Column<VEC> &c) {
+    float f[VEC];
+    c.get(f);
+    shared_store<VEC>(to, f);
+}
+
+// sigmoid with the SFU exp2 and reciprocal (relative error about 2^-21).  A pair shares one reciprocal,
+// 1 / (a b), from which 1 / a = b / (a b): three SFU operations per pair instead of four (they run at
+// an eighth of the issue rate and are the next limit after the issue slots).  The exponent is held
+// at 60 so that a b stays finite; below z = -41 the sigmoid is then 2^-60 instead of less than that.
+__device__ __forceinline__ float sigmoid_fast(float z) {
+    return rcp_approx(1.0f + ex2_approx(fminf(-1.4426950408889634f * z, 60.0f)));
+}
+__device__ __forceinline__ Pair sigmoid_fast(Pair z) {
+    float lo, hi, a, b;
+    split(vmul(z, pair(-1.4426950408889634f, -1.4426950408889634f)), lo, hi);
+    split(vadd(pair(ex2_approx(fminf(lo, 60.0f)), ex2_approx(fminf(hi, 60.0f))), pair(1.0f, 1.0f)), a, b);
+    const float r = rcp_approx(a * b);
+    return vmul(pair(b, a), pair(r, r));
+}
+
+// dy act'(z), silu'(z) = s (1 + z (1 - s)) with s = sigmoid(z).
+template <int ACT, typename E> __device__ __forceinline__ E act_grad(E dy, E z, E one, E minus_one) {
     if (ACT != kActSilu) return dy;
-    const float s = sigmoid_fast(z);
-    return dy * fmaf(z * s, 1.0f - s, s);
+    const E s = sigmoid_fast(z);
+    return vmul(vmul(dy, s), vfma(z, vfma(s, minus_one, one), one));
 }
 
 }  // namespace

@@ -13,6 +13,83 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// ---- sums over the rows of a thread block ----------------------------------------------------------
+// buf[row * ncols + c] summed over `rows` rows into buf[c], pairwise (error of log2(rows) roundings,
+// and the same order on every run).  Synchronises before and after.
+__device__ __forceinline__ void fold_rows(float *buf, int rows, int ncols) {
+    __syncthreads();
+    while (rows > 1) {
+        const int half = (rows + 1) >> 1;
+        const int n = (rows - half) * ncols;
+        for (int i = threadIdx.x; i < n; i += blockDim.x) buf[i] += buf[i + half * ncols];
+        rows = half;
+        __syncthreads();
+    }
+}
+
+// ---- running moments of a thread's column: shifted sums around the first value seen ----------------
+template <int VEC> struct ColumnMoments {
+    float k[VEC], s[VEC], q[VEC];
+    __device__ __forceinline__ void first(const float (&f)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { k[i] = f[i]; s[i] = 0.f; q[i] = 0.f; }
+    }
+    __device__ __forceinline__ void add(const float (&f)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float d = f[i] - k[i];
+            s[i] += d;
+            q[i] = fmaf(d, d, q[i]);
+        }
+    }
+};
+
+// Moments of every column's channels over the block's rows: mean[c] and m2[c] (squared deviations from
+// that mean), c < ncols, out of each thread's n values per channel.  First the means, then the
+// deviations from them as M2_thread + n (mean_thread - mean)^2: only non-negative terms, nothing
+// cancels.  buf: threads * VEC floats, mean: ncols floats; m2 comes back in buf.
+template <int VEC>
+__device__ __forceinline__ void block_moments(const ColumnMoments<VEC> &m, float n, bool active, int row, int rows,
+                                              int col, int ncols, float count, float *buf, float *mean) {
+    __syncthreads();                 // the buffers may still be read from the call before
+    const float inv = n > 0.f ? 1.0f / n : 0.f;
+    float *mine = buf + row * ncols + col * VEC;
+    if (active) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) mine[i] = n > 0.f ? fmaf(n, m.k[i], m.s[i]) : 0.f;
+    }
+    fold_rows(buf, rows, ncols);
+    for (int c = threadIdx.x; c < ncols; c += blockDim.x) mean[c] = buf[c] / count;
+    __syncthreads();
+    if (active) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float t = m.s[i] * inv;
+            const float d = m.k[i] + t - mean[col * VEC + i];
+            mine[i] = n > 0.f ? fmaxf(fmaf(-m.s[i], t, m.q[i]), 0.f) + n * d * d : 0.f;
+        }
+    }
+    fold_rows(buf, rows, ncols);
+}
+
+// ---- per-channel arithmetic ------------------------------------------------------------------------
+// z = (x - pivot) p + q with the mean of the column's first channel as the pivot: where the mean is
+// far from zero compared with the spread, x - pivot loses nothing, and one register serves the vector.
+template <int VEC, int ACT> struct Normalise {
+    float pivot, p[VEC], q[VEC];
+    __device__ __forceinline__ void set(int i, float mean, float rstd, float w, float b) {
+        p[i] = w * rstd;
+        q[i] = fmaf(pivot - mean, p[i], b);
+    }
+    __device__ __forceinline__ void apply(float (&f)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float z = fmaf(f[i] - pivot, p[i], q[i]);
+            f[i] = ACT == kActSilu ? z * sigmoid_fast(z) : z;
+        }
+    }
+};
+
 // Columns are dealt to `col_blocks` thread blocks of `cols` columns each; a block has `rows` rows of threads.
 struct Geometry {
     int vec, columns, col_blocks, cols, rows, splits;
@@ -122,7 +199,8 @@ cl_normalise_kernel(const T *x, T *y, const float2 *__restrict__ stats, const fl
     const Where w = locate(g, hw);
     if (!w.active) return;
     const int width = static_cast<int>(channels / groups);
-    Normalise<T, VEC, ACT> a;
+    Normalise<VEC, ACT> a;
+    a.pivot = stats[w.image * groups + w.channel / width].x;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const float2 st = stats[w.image * groups + (w.channel + i) / width];
@@ -168,7 +246,7 @@ cl_grad_sums_kernel(GnClBackward a, float2 *partial, Geometry g, int64_t hw, int
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float xm = x[i] - mean[i];
-                const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]));
+                const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f, -1.0f);
                 s0[i] += dz;
                 s1[i] = fmaf(dz, xm, s1[i]);
             }
@@ -270,7 +348,7 @@ cl_grad_input_kernel(GnClBackward a, const float2 *__restrict__ group_sums, Geom
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float xm = x[i] - mean[i];
-            const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]));
+            const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f, -1.0f);
             d[i] = fmaf(dz, p[i], -fmaf(xm, c1[i], c0[i]));
         }
         raw_store<T, VEC>(dx + row * channels + w.channel, raw_pack<T, VEC>(d));

@@ -155,6 +155,9 @@ size_t gn_cl_workspace_bytes(const GnClShape &s, bool backward);
 cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void *workspace, cudaStream_t stream);
 cudaError_t gn_cl_backward_launch(const GnClShape &s, const GnClBackward &a, void *workspace, cudaStream_t stream);
 
+// The status word of the channels-last kernels (bit 0: a bounded wait for another block's sums).
+cudaError_t gn_cl_read_status(unsigned int *value, bool clear, cudaStream_t stream);
+
 // ---- 8-bit activation checkpoints (checkpoint.cu; format in ckpt_device.cuh) ---------------------
 cudaError_t ckpt_pack_launch(const void *src, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim,
                              int dtype, cudaStream_t stream);
