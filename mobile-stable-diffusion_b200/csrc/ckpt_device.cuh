@@ -99,10 +99,12 @@ __device__ __forceinline__ uint32_t ckpt_codes(const float (&f)[4], const CkptSc
 }
 
 // Maximum over the 32 / N neighbouring lanes that hold one block (N elements per lane, the first
-// of them on a lane number that is a multiple of 32 / N).  All 32 lanes of the warp take part.
+// of them on a lane number that is a multiple of 32 / N).  Only these lanes have to arrive together.
 template <int N> __device__ __forceinline__ uint32_t block_lanes_max(uint32_t m) {
+    constexpr uint32_t L = kCkptBlock / N;
+    const uint32_t mask = ((1u << L) - 1u) << (threadIdx.x & 31u & ~(L - 1u));
 #pragma unroll
-    for (int o = 1; o < kCkptBlock / N; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (uint32_t o = 1; o < L; o <<= 1) m = max(m, __shfl_xor_sync(mask, m, o));
     return m;
 }
 

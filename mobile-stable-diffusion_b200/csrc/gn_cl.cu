@@ -14,10 +14,6 @@ bool vectors_ok(const void *a, const void *b, const void *c) {
     return aligned(a, 16) && aligned(b, 16) && aligned(c, 16);
 }
 
-// codes by the vector, scales by the word
-bool checkpoint_ok(const GnClShape &s, const void *codes, const void *scales) {
-    return aligned(codes, s.dtype == kF32 ? 4 : 8) && aligned(scales, 4);
-}
 
 }  // namespace
 
@@ -34,7 +30,7 @@ size_t gn_cl_workspace_bytes(const GnClShape &s, bool backward) {
 cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void *ws, cudaStream_t stream) {
     const bool vectors = vectors_ok(a.in, a.out, nullptr);
     GnClTeamPlan p;
-    if (a.codes && vectors && checkpoint_ok(s, a.codes, a.scales) && gn_cl_team_plan(s, true, false, false, &p))
+    if (a.codes && vectors && aligned(a.codes, s.dtype == kF32 ? 4 : 8) && gn_cl_team_plan(s, true, false, false, &p))
         return gn_cl_team_forward(s, p, a, ws, stream);
     GnClForward norm = a;
     if (a.codes) {                                     // two steps, the checkpoint first: out may be in
@@ -49,7 +45,7 @@ cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void 
 
 cudaError_t gn_cl_backward_launch(const GnClShape &s, const GnClBackward &a, void *ws, cudaStream_t stream) {
     GnClTeamPlan p;
-    if (vectors_ok(a.in, a.grad_out, a.grad_in) && checkpoint_ok(s, a.codes, a.scales) &&
+    if (vectors_ok(a.in, a.grad_out, a.grad_in) && aligned(a.codes, 16) &&
         gn_cl_team_plan(s, false, true, a.codes != nullptr, &p))
         return gn_cl_team_backward(s, p, a, ws, stream);
     return gn_cl_split_backward(s, a, ws, stream);

@@ -133,6 +133,19 @@ template <> struct Column<1> {
     __device__ __forceinline__ void get(float *f) const { f[0] = e[0]; }
 };
 
+// The codes of a column as whole numbers; times the step they are the values (exact either way).
+__device__ __forceinline__ void codes4(uint32_t w, Pair &lo, Pair &hi) {
+    const Pair offset = pair(-8388736.0f, -8388736.0f);
+    w ^= 0x80808080u;
+    lo = vadd(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540u)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541u))), offset);
+    hi = vadd(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7542u)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7543u))), offset);
+}
+__device__ __forceinline__ void code_column(const uint2 &w, Column<8> &c) {
+    codes4(w.x, c.e[0], c.e[1]);
+    codes4(w.y, c.e[2], c.e[3]);
+}
+__device__ __forceinline__ void code_column(uint32_t w, Column<4> &c) { codes4(w, c.e[0], c.e[1]); }
+
 // VEC floats of shared memory, 16 bytes at a time (rows of a thread's column are 16-byte aligned).
 template <int VEC> __device__ __forceinline__ void shared_store(float *to, const float (&f)[VEC]) {
     if constexpr (VEC == 1) to[0] = f[0];
@@ -174,7 +187,7 @@ __device__ __forceinline__ Pair sigmoid_fast(Pair z) {
     split(vmul(z, pair(-1.4426950408889634f, -1.4426950408889634f)), lo, hi);
     split(vadd(pair(ex2_approx(fminf(lo, 60.0f)), ex2_approx(fminf(hi, 60.0f))), pair(1.0f, 1.0f)), a, b);
     const float r = rcp_approx(a * b);
-    return vmul(pair(b, a), pair(r, r));
+    return pair(b * r, a * r);
 }
 
 // dy act'(z), silu'(z) = s (1 + z (1 - s)) with s = sigmoid(z).

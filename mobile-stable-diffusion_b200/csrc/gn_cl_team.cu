@@ -13,10 +13,12 @@
 // second read comes from L2 whatever the tensor's size.  A team with more than one item runs S of the
 // next item between S and A of the current one, which hides the exchange.
 //
-// Loads.  Every thread owns a ring of 16-byte slots in shared memory that it fills by cp.async a few
-// chunks ahead of its own use, so no barrier guards the ring.  The ring runs on over the end of a
-// pass: while a block adds up its rows and waits for the others' sums, the first chunks of the next
-// pass are already under way.
+// Loads.  A producer warp keeps a ring of chunks filled by tiled bulk copies (a chunk is kRounds rows per
+// consumer thread, the box of a 2-D tensor map over [batch * hw, channels]); the consumer warps wait on
+// a chunk's "full" mbarrier and release it through its "empty" one.  The ring runs on over the end of
+// a pass: while a block adds up its rows and waits for the others' sums, the first chunks of the next
+// pass are already under way.  The copies cost the consumers no issue slots, and those are what the
+// gradient runs short of first (per-thread cp.async into the same ring: 12 more instructions per vector).
 //
 // Exchange.  A block writes its sums per group to the workspace and counts itself in; before pass A every
 // block polls the count and merges all of the team's sums itself, in block order (the same bits on
@@ -27,6 +29,9 @@
 // writes them once per slice; cl_param_sum_kernel adds the blocks' rows.
 #include "gn_cl_device.cuh"
 #include "gn_cl_internal.h"
+#include "gn_device.cuh"
+
+#include <cuda.h>
 
 #include <algorithm>
 #include <numeric>
@@ -35,18 +40,15 @@ namespace sdfl {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;                      // consumers
 constexpr int kWarps = kThreads / 32;
-constexpr int kBlocksPerSm = 3;
-constexpr int kBlocksPerSmGrad = 2;
-// ring: chunks of kChunk vectors per thread, kStages chunks deep (the backward pass has two tensors)
-constexpr int kChunk = 4, kStages = 3;
-constexpr int kChunkGrad = 2, kStagesGrad = 4;
-constexpr int kMaxCols = kThreads / 2;             // columns of a slice: keeps shared memory under 48 KB
-constexpr int kMaxMembers = 512;
-constexpr int kMergeLoads = kMaxMembers / 32;
+constexpr int kBlock = kThreads + 32;              // and the producer warp
+constexpr int kBlocksPerSm = 2;
+constexpr int kRounds = 2;                         // rows per thread and chunk
+constexpr int kStages = 6, kStagesGrad = 5;        // chunks of the ring: 8 KB per tensor each
+constexpr int kMaxCols = kThreads / 2;             // columns of a slice: a box row of 2 KB
+constexpr int kMergeLoads = 5;                     // a team of up to 160 blocks in one round
 constexpr int64_t kInFlight = 64ll << 20;
-constexpr long long kWaitCycles = 2000000000LL;    // about a second
 
 __device__ unsigned int g_cl_status;               // bit 0: a bounded wait ran out
 
@@ -56,7 +58,8 @@ struct Args {                    // one struct for both directions
     GnClTeamPlan p;
     int64_t batch, hw, channels, groups;
     int width;                   // channels per group
-    int share, rest;             // pixels / members, pixels % members
+    int chunk_rows;              // pixels per chunk
+    int share, rest;             // chunks of an image / members, % members
     float eps;
     unsigned int *arrived;       // [items]
     float2 *partial;             // [batch * groups][members]
@@ -65,12 +68,18 @@ struct Args {                    // one struct for both directions
 
 struct Place {
     int member, slice_team, image_team, col, row, ncols, slice_groups;
-    int64_t first;               // this block's pixels of every item: [first, first + pixels)
-    int pixels, mine;            // of those, this thread's rows: row, row + rows, ...
+    int first, chunks, pixels;   // this block's pixels of every item: [first, first + pixels)
     bool active;
 };
 
-__device__ __forceinline__ int member_pixels(const Args &a, int member) { return a.share + (member < a.rest ? 1 : 0); }
+// A block's share of an item is whole chunks; the image's last chunk may be short.
+__device__ __forceinline__ int member_first(const Args &a, int member) {
+    return (member * a.share + min(member, a.rest)) * a.chunk_rows;
+}
+__device__ __forceinline__ int member_pixels(const Args &a, int member) {
+    const int first = member_first(a, member);
+    return min(static_cast<int>(a.hw) - first, (a.share + (member < a.rest ? 1 : 0)) * a.chunk_rows);
+}
 
 __device__ __forceinline__ Place place(const Args &a) {
     Place w;
@@ -83,61 +92,104 @@ __device__ __forceinline__ Place place(const Args &a) {
     w.active = w.row < a.p.rows;
     w.ncols = a.p.cols * a.p.vec;
     w.slice_groups = w.ncols / a.width;
-    w.first = static_cast<int64_t>(w.member) * a.share + min(w.member, a.rest);
+    w.first = member_first(a, w.member);
+    w.chunks = a.share + (w.member < a.rest ? 1 : 0);
     w.pixels = member_pixels(a, w.member);
-    w.mine = w.active ? (w.pixels - w.row + a.p.rows - 1) / a.p.rows : 0;
     return w;
 }
 
-// A team's items, slice by slice and image by image within a slice, and the order of their passes:
-// S0, then S1 A0, S2 A1, ... and the last A (a team of one block, which has nobody to wait for: S0 A0 S1 A1 ...).
-struct Items {
-    int count, images, slice0, slice_step, image0, image_step;
-    bool lag;
-    __device__ __forceinline__ Items(const Args &a, const Place &w) {
-        images = (static_cast<int>(a.batch) - w.image_team + a.p.image_teams - 1) / a.p.image_teams;
-        count = images * ((a.p.slices - w.slice_team + a.p.slice_teams - 1) / a.p.slice_teams);
-        slice0 = w.slice_team;
-        slice_step = a.p.slice_teams;
-        image0 = w.image_team;
-        image_step = a.p.image_teams;
-        lag = a.p.members > 1;
-    }
-    __device__ __forceinline__ int slice(int k) const { return slice0 + (k / images) * slice_step; }
-    __device__ __forceinline__ int64_t image(int k) const { return image0 + (k % images) * image_step; }
-    __device__ __forceinline__ int passes() const { return 2 * count; }
-    // pass number -> item, and whether it is the second pass
-    __device__ __forceinline__ int item(int pass, bool *second) const {
-        if (!lag) {
-            *second = pass & 1;
-            return pass >> 1;
+// A team's items, slice by slice and image by image within a slice.
+struct Cursor {
+    int slice, image;
+    __device__ __forceinline__ void next(const Args &a, const Place &w) {
+        image += a.p.image_teams;
+        if (image >= static_cast<int>(a.batch)) {
+            image = w.image_team;
+            slice += a.p.slice_teams;
         }
-        *second = pass > 0 && ((pass & 1) == 0 || pass == 2 * count - 1);
-        if (!*second) return (pass + 1) >> 1;
-        return pass == 2 * count - 1 ? count - 1 : (pass >> 1) - 1;
     }
 };
 
-__device__ __forceinline__ void copy_async16(void *to, const void *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
-                 : "memory");
+// The order of a team's passes: S0 A0 S1 A1 ..., or with a lag S0, S1 A0, S2 A1, ... and the last A.
+struct Passes {
+    Cursor s, a, now;
+    bool lag, sum_next, second;
+    __device__ __forceinline__ Passes(const Args &args, const Place &w) {
+        s = a = now = Cursor{w.slice_team, w.image_team};
+        lag = args.p.lag == 1 || (args.p.lag == 2 && ((w.image_team * args.p.slice_teams + w.slice_team) & 1));
+        sum_next = true;
+        second = false;
+    }
+    // false: none left
+    __device__ __forceinline__ bool next(const Args &args, const Place &w) {
+        const bool more = s.slice < args.p.slices;
+        if (!more && a.slice >= args.p.slices) return false;
+        if (more && sum_next) {
+            second = false;
+            now = s;
+            s.next(args, w);
+            sum_next = lag;                           // once: one S ahead from here on
+            lag = false;
+        } else {
+            second = sum_next = true;
+            now = a;
+            a.next(args, w);
+        }
+        return true;
+    }
+};
+
+// One box of a tensor map into shared memory; x in 8-byte units (even: 16-byte aligned), y a pixel row.
+__device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3}], [%4], %5;"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "l"(policy)
+        : "memory");
 }
-__device__ __forceinline__ void copy_async8(void *to, const void *from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
-                 : "memory");
-}
-// 4 bytes, of which only the first `bytes` are read (the rest is zero-filled)
-__device__ __forceinline__ void copy_async4(void *to, const void *from, uint32_t bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                 "l"(from), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The ring's barriers; waits are bounded, a time-out is recorded and the block carries on.
+template <int STAGES> struct Ring {
+    uint32_t full, empty;        // shared addresses of STAGES mbarriers each
+    int stage;
+    uint32_t phase;
+    __device__ __forceinline__ void init(uint64_t *bars) {
+        full = smem_addr(bars);
+        empty = full + 8 * STAGES;
+        stage = 0;
+        phase = 0;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < STAGES; ++i) {
+                mbar_init(full + 8 * i, 1);
+                mbar_init(empty + 8 * i, kWarps);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
+        if (!mbar_wait_bounded(bar + 8 * stage, parity, kWaitCycles)) atomicOr(&g_cl_status, 1u);
+    }
+    __device__ __forceinline__ void wait_full() { wait(full, phase); }
+    __device__ __forceinline__ void wait_empty() { wait(empty, phase ^ 1u); }
+    // a consumer warp has read its part of the chunk
+    __device__ __forceinline__ void release() {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(empty + 8 * stage);
+        next();
+    }
+    __device__ __forceinline__ void next() {
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+__device__ __forceinline__ void block_sync() { consumer_sync(kThreads); }       // the consumer warps
 
 // Counts the block in on an item; its sums were written (by any thread) before.
 __device__ __forceinline__ void arrive(const Args &a, int64_t item) {
-    __syncthreads();
+    block_sync();
     if (threadIdx.x == 0) {
         __threadfence();
         atomicAdd(a.arrived + item, 1u);
@@ -158,16 +210,16 @@ __device__ __forceinline__ void wait_all(const Args &a, int64_t item) {
             }
         }
     }
-    __syncthreads();
+    block_sync();
 }
 
-// One group's sums of all the team's blocks, 32 per round, every load in flight at once.
-__device__ __forceinline__ void load_partials(const Args &a, int64_t group, int lane, float2 (&v)[kMergeLoads]) {
-    const float2 *q = a.partial + group * a.p.members;
+// One group's sums of all the team's blocks, kMergeLoads * 32 per round with every load in flight at once.
+__device__ __forceinline__ void load_partials(const Args &a, int64_t group, int first, float2 (&v)[kMergeLoads]) {
+    const float2 *q = a.partial + group * a.p.members + first;
 #pragma unroll
     for (int k = 0; k < kMergeLoads; ++k) {
         v[k] = make_float2(0.f, 0.f);
-        if (lane + 32 * k < a.p.members) v[k] = __ldcg(q + lane + 32 * k);
+        if (first + 32 * k < a.p.members) v[k] = __ldcg(q + 32 * k);
     }
 }
 __device__ __forceinline__ float pixels_or_none(const Args &a, int member) {
@@ -194,7 +246,7 @@ struct Segments {
 // buf[row][ncols], filled by every active thread, to buf[c] = sum over the rows, in a fixed order: each
 // thread adds rows of one column, `parts` threads per column.  Synchronises before and after.
 __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
-    __syncthreads();
+    block_sync();
     if (ncols >= kThreads) {
         for (int c = threadIdx.x; c < ncols; c += kThreads) {
             float s = buf[c];
@@ -210,9 +262,9 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
             for (int r = part; r < rows; r += parts) s += buf[r * ncols + c];
         }
         if (parts > 1) {
-            __syncthreads();
+            block_sync();
             if (part > 0 && part < parts) buf[threadIdx.x] = s;
-            __syncthreads();
+            block_sync();
             if (part == 0) {
                 for (int k = 1; k < parts; ++k) s += buf[k * ncols + c];
                 buf[c] = s;
@@ -221,7 +273,7 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
             buf[c] = s;
         }
     }
-    __syncthreads();
+    block_sync();
 }
 
 // ---- forward --------------------------------------------------------------------------------------
@@ -231,99 +283,107 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
 // outlier's share of one thread's pixels, which costs at most log2(rows) bits), so the one
 // subtraction that is left, of N (block mean - P)^2, cancels next to nothing.
 template <typename T, int ACT, bool PACK>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-cl_team_forward_kernel(const Args a) {
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm)
+cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) {
     constexpr int VEC = VecOf<T>::N;
+    constexpr int kChunkBytes = kRounds * kThreads * 16;
     using Col = Column<VEC>;
-    extern __shared__ __align__(16) unsigned char shared[];
+    extern __shared__ __align__(128) unsigned char shared[];
+    __shared__ uint64_t bars[2 * kStages];
     const Place w = place(a);
-    uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;                       // [slot][thread]
-    float *buf = reinterpret_cast<float *>(shared + kChunk * kStages * kThreads * 16);   // [rows][2 ncols]
+    float *buf = reinterpret_cast<float *>(shared + kStages * kChunkBytes);              // [rows][2 ncols]
     float *cp = buf + 2 * kThreads * VEC;             // [ncols] each: P, later the scale; shift; minus the pivots
     float *cq = cp + w.ncols;
     float *pivots = cq + w.ncols;
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (mean, rstd)
+    int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Passes passes(a, w);
+    Ring<kStages> ring;
+    ring.init(bars);
+    for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
+    __syncthreads();
+
+    if (warp == kWarps) {                             // producer
+        if (lane == 0) {
+            const uint64_t again = policy_evict_last(), done = policy_evict_first();
+            const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols * sizeof(T));
+            while (passes.next(a, w)) {
+                const int x = static_cast<int>(passes.now.slice * w.ncols * sizeof(T) / 8);
+                const int y = passes.now.image * static_cast<int>(a.hw) + w.first;
+                for (int c = 0; c < w.chunks; ++c, ring.next()) {
+                    ring.wait_empty();
+                    mbar_expect_tx(ring.full + 8 * ring.stage, bytes);
+                    box_load(smem_addr(shared) + ring.stage * kChunkBytes, &map_x, x, y + c * a.chunk_rows,
+                             ring.full + 8 * ring.stage, passes.second ? done : again);
+                }
+            }
+        }
+        return;
+    }
+
     const Segments seg(a.width);
-    const T *x = static_cast<const T *>(a.f.in);
     T *y = static_cast<T *>(a.f.out);
     const int64_t step = static_cast<int64_t>(a.p.rows) * a.channels;
     const int64_t mine0 = (w.first + w.row) * a.channels + w.col * VEC;                 // within an image, slice 0
-    const int chunks = ((w.pixels + a.p.rows - 1) / a.p.rows + kChunk - 1) / kChunk;     // per pass
-    const Items items(a, w);
-
-    // the loading end of the ring
-    const T *src = nullptr;
-    int pass = -1, chunks_left = 0, left = 0, in = 0;
-    auto load_chunk = [&]() {
-        if (chunks_left == 0 && pass + 1 < items.passes()) {
-            bool second;
-            const int k = items.item(++pass, &second);
-            src = x + items.image(k) * a.hw * a.channels + items.slice(k) * w.ncols + mine0;
-            chunks_left = chunks;
-            left = w.mine;
-        }
-        if (chunks_left > 0) {
+    // this thread's vectors within a chunk, and its rows of a pass
+    const uint4 *mine_in = reinterpret_cast<const uint4 *>(shared) + (w.active ? w.row * a.p.cols + w.col : 0);
+    const int round = a.p.rows * a.p.cols;
+    const int mine = w.active ? (w.pixels - w.row + a.p.rows - 1) / a.p.rows : 0;
+    // one(vector) for each of them
+    auto each = [&](auto one) {
+        int left = mine;
+        for (int c = 0; c < w.chunks; ++c, left -= kRounds) {
+            ring.wait_full();
+            const uint4 *p = mine_in + ring.stage * (kChunkBytes / 16);
+            uint4 v[kRounds];
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k)
-                if (k < left) copy_async16(ring + (in + k) * kThreads, src + k * step);
-            src += kChunk * step;
-            left -= kChunk;
-            --chunks_left;
-            in = in == kChunk * (kStages - 1) ? 0 : in + kChunk;
-        }
-        copy_commit();
-    };
-    int out = 0;
-    auto take_chunk = [&](uint4 (&v)[kChunk]) {
-        copy_wait<kStages - 1>();
+            for (int k = 0; k < kRounds; ++k) v[k] = p[k * round];
+            ring.release();
+            if (left >= kRounds) {
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) v[k] = ring[(out + k) * kThreads];
-        out = out == kChunk * (kStages - 1) ? 0 : out + kChunk;
-        load_chunk();
+                for (int k = 0; k < kRounds; ++k) one(v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kRounds; ++k)
+                    if (k < left) one(v[k]);
+            }
+        }
     };
 
     auto sums = [&](int slice, int64_t image) {
         Col nk, s, q;                                 // minus the first value, sum, sum of squares
 #pragma unroll
         for (int i = 0; i < Col::N; ++i) { nk.e[i] = Col::all(0.f); s.e[i] = Col::all(0.f); q.e[i] = Col::all(0.f); }
-        int64_t at = image * a.hw * a.channels + slice * w.ncols + mine0;
-        for (int r = 0; r < chunks * kChunk; r += kChunk, at += kChunk * step) {
-            uint4 v[kChunk];
-            take_chunk(v);
+        if (mine) {
+            ring.wait_full();
+            float f[VEC];
+            unpack<T>(mine_in[ring.stage * (kChunkBytes / 16)], f);
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k) {
-                float f[VEC];
-                unpack<T>(v[k], f);
-                if constexpr (PACK) {
-                    // lanes past the end hold stale values of other rows, but never those of a live block
-                    const CkptScale sc = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
-                    if (r + k < w.mine) {
-                        *reinterpret_cast<typename CodeVec<VEC>::type *>(a.f.codes + at + k * step) = ckpt_codes(f, sc);
-                        if ((w.col & (kCkptBlock / VEC - 1)) == 0)
-                            a.f.scales[(at + k * step) / kCkptBlock] = static_cast<uint8_t>(sc.e);
-                    }
-                }
-                if (r + k < w.mine) {
-                    if (k == 0 && r == 0) {
-                        float g[VEC];
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) g[i] = -f[i];
-                        nk.set(g);
-                    }
-                    Col c;
-                    c.set(f);
-#pragma unroll
-                    for (int i = 0; i < Col::N; ++i) {
-                        const Pair d = vadd(c.e[i], nk.e[i]);
-                        s.e[i] = vadd(s.e[i], d);
-                        q.e[i] = vfma(d, d, q.e[i]);
-                    }
-                }
-            }
+            for (int i = 0; i < VEC; ++i) f[i] = -f[i];
+            nk.set(f);
         }
+        int64_t at = image * a.hw * a.channels + slice * w.ncols + mine0;
+        each([&](const uint4 &v) {
+            float f[VEC];
+            unpack<T>(v, f);
+            if constexpr (PACK) {
+                const CkptScale sc = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
+                *reinterpret_cast<typename CodeVec<VEC>::type *>(a.f.codes + at) = ckpt_codes(f, sc);
+                if ((w.col & (kCkptBlock / VEC - 1)) == 0) a.f.scales[at / kCkptBlock] = static_cast<uint8_t>(sc.e);
+                at += step;
+            }
+            Col c;
+            c.set(f);
+#pragma unroll
+            for (int i = 0; i < Col::N; ++i) {
+                const Pair d = vadd(c.e[i], nk.e[i]);
+                s.e[i] = vadd(s.e[i], d);
+                q.e[i] = vfma(d, d, q.e[i]);
+            }
+        });
         // block sums
-        const float n = static_cast<float>(w.mine), inv = w.mine ? 1.0f / n : 0.f;
+        const float n = static_cast<float>(mine), inv = mine ? 1.0f / n : 0.f;
         float mean[VEC], m2[VEC];
         {
             float k[VEC], t[VEC], u[VEC];
@@ -335,18 +395,18 @@ cl_team_forward_kernel(const Args a) {
                 m2[i] = fmaxf(fmaf(-t[i], shift, u[i]), 0.f);
             }
         }
-        __syncthreads();                              // the buffers may still be read by the pass before
+        block_sync();                              // the buffers may still be read by the pass before
         if (w.row == 0) shared_store<VEC>(cp + w.col * VEC, mean);
-        __syncthreads();
+        block_sync();
         if (w.active) {
             float *to = buf + w.row * 2 * w.ncols + w.col * VEC;
             float head[VEC];
             shared_load<VEC>(cp + w.col * VEC, head);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = w.mine ? mean[i] - head[i] : 0.f;
+                const float d = mine ? mean[i] - head[i] : 0.f;
                 mean[i] = n * d;
-                m2[i] = w.mine ? fmaf(n * d, d, m2[i]) : 0.f;
+                m2[i] = mine ? fmaf(n * d, d, m2[i]) : 0.f;
             }
             shared_store<VEC>(to, mean);
             shared_store<VEC>(to + w.ncols, m2);
@@ -379,19 +439,32 @@ cl_team_forward_kernel(const Args a) {
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float hw = static_cast<float>(a.hw), width = static_cast<float>(a.width);
         for (int g = warp; g < w.slice_groups; g += kWarps) {
-            float2 v[kMergeLoads];
-            load_partials(a, group0 + g, lane, v);
-            float t = 0.f;
+            // Chan's merge, round by round of up to 160 blocks
+            float mu = 0.f, u = 0.f, n = 0.f;
+            for (int first = 0; first < a.p.members; first += 32 * kMergeLoads) {
+                float2 v[kMergeLoads];
+                load_partials(a, group0 + g, first + lane, v);
+                float t = 0.f, px = 0.f;
 #pragma unroll
-            for (int k = 0; k < kMergeLoads; ++k) t = fmaf(pixels_or_none(a, lane + 32 * k), v[k].x, t);
-            const float mu = warp_sum(t) / hw;
-            float u = 0.f;
+                for (int k = 0; k < kMergeLoads; ++k) {
+                    const float c = pixels_or_none(a, first + lane + 32 * k);
+                    t = fmaf(c, v[k].x, t);
+                    px += c;
+                }
+                px = warp_sum(px);
+                const float m = warp_sum(t) / px;
+                float e = 0.f;
 #pragma unroll
-            for (int k = 0; k < kMergeLoads; ++k) {
-                const float d = v[k].x - mu;
-                u += fmaf(pixels_or_none(a, lane + 32 * k) * width * d, d, v[k].y);
+                for (int k = 0; k < kMergeLoads; ++k) {
+                    const float d = v[k].x - m;
+                    e += fmaf(pixels_or_none(a, first + lane + 32 * k) * width * d, d, v[k].y);
+                }
+                e = warp_sum(e);
+                const float d = m - mu, f = px / (n + px);
+                u += e + d * d * n * width * f;
+                mu = fmaf(d, f, mu);
+                n += px;
             }
-            u = warp_sum(u);
             if (lane == 0) {
                 const float rstd = 1.0f / sqrtf(u / (hw * width) + a.eps);
                 stat[g] = make_float2(mu, rstd);
@@ -401,68 +474,59 @@ cl_team_forward_kernel(const Args a) {
                 }
             }
         }
-        __syncthreads();
+        block_sync();
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
             const int channel = slice * w.ncols + c;
-            const float2 st = stat[c / a.width];
-            const float pivot = stat[(c - c % VEC) / a.width].x;
+            const float2 st = stat[group_of[c]];
+            const float pivot = stat[group_of[c - c % VEC]].x;
             const float scale = a.f.gamma[channel] * st.y;
             cp[c] = scale;
             cq[c] = fmaf(pivot - st.x, scale, a.f.beta[channel]);
             pivots[c] = -pivot;
         }
-        __syncthreads();
+        block_sync();
         Col cs, ch;
-        column_load<VEC>(cp + w.col * VEC, cs);
-        column_load<VEC>(cq + w.col * VEC, ch);
-        const Pair np = Col::all(pivots[w.col * VEC]);
+        const int col = w.active ? w.col * VEC : 0;
+        column_load<VEC>(cp + col, cs);
+        column_load<VEC>(cq + col, ch);
+        const Pair np = Col::all(pivots[col]);
         T *o = y + image * a.hw * a.channels + slice * w.ncols + mine0;
-        for (int r = 0; r < chunks * kChunk; r += kChunk, o += kChunk * step) {
-            uint4 v[kChunk];
-            take_chunk(v);
+        each([&](const uint4 &v) {
+            float f[VEC];
+            unpack<T>(v, f);
+            Col c;
+            c.set(f);
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k)
-                if (r + k < w.mine) {
-                    float f[VEC];
-                    unpack<T>(v[k], f);
-                    Col c;
-                    c.set(f);
-#pragma unroll
-                    for (int i = 0; i < Col::N; ++i) {
-                        const Pair z = vfma(vadd(c.e[i], np), cs.e[i], ch.e[i]);
-                        c.e[i] = ACT == kActSilu ? vmul(z, sigmoid_fast(z)) : z;
-                    }
-                    c.get(f);
-                    st_stream(o + k * step, pack<T>(f));
-                }
-        }
+            for (int i = 0; i < Col::N; ++i) {
+                const Pair z = vfma(vadd(c.e[i], np), cs.e[i], ch.e[i]);
+                c.e[i] = ACT == kActSilu ? vmul(z, sigmoid_fast(z)) : z;
+            }
+            c.get(f);
+            st_stream(o, pack<T>(f));
+            o += step;
+        });
     };
 
-    for (int k = 0; k < kStages; ++k) load_chunk();
-    for (int p = 0; p < items.passes(); ++p) {
-        bool second;
-        const int k = items.item(p, &second);
-        if (second) apply(items.slice(k), items.image(k));
-        else sums(items.slice(k), items.image(k));
+    while (passes.next(a, w)) {
+        if (passes.second) apply(passes.now.slice, passes.now.image);
+        else sums(passes.now.slice, passes.now.image);
     }
 }
 
 // ---- backward -------------------------------------------------------------------------------------
 template <typename T, int ACT, bool CKPT>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSmGrad)
-cl_team_backward_kernel(const Args a) {
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm)
+cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy) {
     constexpr int VEC = VecOf<T>::N;
-    constexpr int kSlots = kChunkGrad * kStagesGrad;
+    constexpr int kBytes = kRounds * kThreads * 16;                  // grad_out's part of a chunk
+    constexpr int kBytesX = CKPT ? kRounds * kThreads * VEC : kBytes;
+    constexpr int kChunkBytes = kBytes + kBytesX;
     using Col = Column<VEC>;
-    using Codes = typename CodeVec<VEC>::type;
-    extern __shared__ __align__(16) unsigned char shared[];
+    using X = std::conditional_t<CKPT, typename CodeVec<VEC>::type, uint4>;
+    extern __shared__ __align__(128) unsigned char shared[];
+    __shared__ uint64_t bars[2 * kStagesGrad];
     const Place w = place(a);
-    uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;                       // grad_out, [slot][thread]
-    unsigned char *ring2 = shared + kSlots * kThreads * 16;                              // x, or codes and scale words
-    uint4 *ring_x = reinterpret_cast<uint4 *>(ring2) + threadIdx.x;
-    Codes *ring_c = reinterpret_cast<Codes *>(ring2) + threadIdx.x;
-    uint32_t *ring_s = reinterpret_cast<uint32_t *>(ring2 + kSlots * kThreads * sizeof(Codes)) + threadIdx.x;
-    float *buf = reinterpret_cast<float *>(ring2 + kSlots * kThreads * 16);              // [rows][2 ncols]
+    float *buf = reinterpret_cast<float *>(shared + kStagesGrad * kChunkBytes);          // [rows][2 ncols]
     float *total = buf + 2 * kThreads * VEC;          // [2 ncols]: this slice's channel sums over the images
     float *cp = total + 2 * w.ncols;                  // [ncols] each: scale and shift of z; c0 and c1; minus the pivots
     float *cq = cp + w.ncols;
@@ -470,99 +534,138 @@ cl_team_backward_kernel(const Args a) {
     float *c1 = c0 + w.ncols;
     float *pivots = c1 + w.ncols;
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (s1, s2)
+    int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Passes passes(a, w);
+    Ring<kStagesGrad> ring;
+    ring.init(bars);
+    for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
+    __syncthreads();
+
+    if (warp == kWarps) {                             // producer
+        if (lane == 0) {
+            const uint64_t again = policy_evict_last(), done = policy_evict_first();
+            constexpr int kSizeX = CKPT ? 1 : sizeof(T);
+            const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols) * (sizeof(T) + kSizeX);
+            while (passes.next(a, w)) {
+                const int x = static_cast<int>(passes.now.slice * w.ncols * sizeof(T) / 8);
+                const int xx = passes.now.slice * w.ncols * kSizeX / 8;
+                const int y = passes.now.image * static_cast<int>(a.hw) + w.first;
+                const uint64_t policy = passes.second ? done : again;
+                for (int c = 0; c < w.chunks; ++c, ring.next()) {
+                    ring.wait_empty();
+                    const uint32_t bar = ring.full + 8 * ring.stage, to = smem_addr(shared) + ring.stage * kChunkBytes;
+                    mbar_expect_tx(bar, bytes);
+                    box_load(to, &map_dy, x, y + c * a.chunk_rows, bar, policy);
+                    box_load(to + kBytes, &map_x, xx, y + c * a.chunk_rows, bar, policy);
+                }
+            }
+        }
+        return;
+    }
+
     const Segments seg(a.width);
-    const int64_t blocks_row = ckpt_blocks(a.channels), scale_bytes = a.batch * a.hw * blocks_row;
-    const T *x = static_cast<const T *>(a.b.in);
-    const T *dy = static_cast<const T *>(a.b.grad_out);
+    const int64_t blocks_row = ckpt_blocks(a.channels), scale_step = a.p.rows * blocks_row;
     T *dx = static_cast<T *>(a.b.grad_in);
     const Pair one = Col::all(1.0f), minus_one = Col::all(-1.0f);
     const int64_t step = static_cast<int64_t>(a.p.rows) * a.channels;
     const int64_t mine0 = (w.first + w.row) * a.channels + w.col * VEC;
-    const int chunks = ((w.pixels + a.p.rows - 1) / a.p.rows + kChunkGrad - 1) / kChunkGrad;
-    const Items items(a, w);
-
-    int64_t src = 0, scale_at = 0;                    // element, scale byte
-    int pass = -1, chunks_left = 0, left = 0, in = 0;
-    auto load_chunk = [&]() {
-        if (chunks_left == 0 && pass + 1 < items.passes()) {
-            bool second;
-            const int k = items.item(++pass, &second);
-            const int channel = items.slice(k) * w.ncols + w.col * VEC;
-            src = items.image(k) * a.hw * a.channels + items.slice(k) * w.ncols + mine0;
-            scale_at = (items.image(k) * a.hw + w.first + w.row) * blocks_row + channel / kCkptBlock;
-            chunks_left = chunks;
-            left = w.mine;
-        }
-        if (chunks_left > 0) {
+    // this thread's vectors within a chunk, and its rows of a pass
+    const int place_in = w.active ? w.row * a.p.cols + w.col : 0;
+    const int round = a.p.rows * a.p.cols;
+    const int mine = w.active ? (w.pixels - w.row + a.p.rows - 1) / a.p.rows : 0;
+    // The scale bytes of a checkpoint (less than 16 bytes a row) are loaded into registers one chunk ahead.
+    const uint8_t *scale_at = nullptr;
+    uint8_t scale[kRounds] = {};
+    auto load_scales = [&](int left) {
+        if constexpr (CKPT) {
 #pragma unroll
-            for (int k = 0; k < kChunkGrad; ++k)
-                if (k < left) {
-                    const int slot = (in + k) * kThreads;
-                    copy_async16(ring + slot, dy + src + k * step);
-                    if constexpr (CKPT) {
-                        if constexpr (VEC == 8) copy_async8(ring_c + slot, a.b.codes + src + k * step);
-                        else copy_async4(ring_c + slot, a.b.codes + src + k * step, 4);
-                        // the aligned word that holds the scale byte, or what there is of it
-                        const int64_t word = (scale_at + k * a.p.rows * blocks_row) & ~static_cast<int64_t>(3);
-                        const int64_t rest = scale_bytes - word;
-                        copy_async4(ring_s + slot, a.b.scales + word, rest < 4 ? static_cast<uint32_t>(rest) : 4u);
-                    } else {
-                        copy_async16(ring_x + slot, x + src + k * step);
-                    }
-                }
-            src += kChunkGrad * step;
-            scale_at += static_cast<int64_t>(kChunkGrad) * a.p.rows * blocks_row;
-            left -= kChunkGrad;
-            --chunks_left;
-            in = in == kSlots - kChunkGrad ? 0 : in + kChunkGrad;
+            for (int k = 0; k < kRounds; ++k)
+                if (k < left) scale[k] = scale_at[k * scale_step];
+            scale_at += kRounds * scale_step;
         }
-        copy_commit();
     };
-    // x and grad_out of the next chunk; `at` is the scale byte of its first row
-    int out = 0;
-    auto take_chunk = [&](Col (&xc)[kChunkGrad], Col (&dc)[kChunkGrad], int64_t at) {
-        copy_wait<kStagesGrad - 1>();
-#pragma unroll
-        for (int k = 0; k < kChunkGrad; ++k) {
-            const int slot = (out + k) * kThreads;
-            float f[VEC];
-            unpack<T>(ring[slot], f);
-            dc[k].set(f);
-            if constexpr (CKPT) {
-                const uint32_t shift = static_cast<uint32_t>(at + k * a.p.rows * blocks_row) & 3u;
-                const uint8_t e = static_cast<uint8_t>(ring_s[slot] >> (8 * shift));
-                ckpt_values(ring_c[slot], ckpt_step(e), f);
-            } else {
-                unpack<T>(ring_x[slot], f);
-            }
-            xc[k].set(f);
+    auto first_scales = [&](int slice, int64_t image) {
+        if constexpr (CKPT) {
+            scale_at = a.b.scales + (image * a.hw + w.first + w.row) * blocks_row +
+                       (slice * w.ncols + w.col * VEC) / kCkptBlock;
+            load_scales(mine);
         }
-        out = out == kSlots - kChunkGrad ? 0 : out + kChunkGrad;
-        load_chunk();
+    };
+    // x - pivot
+    auto shifted = [&](const X &v, uint8_t e, Pair np, Col &xm) {
+        if constexpr (CKPT) {
+            code_column(v, xm);
+            const Pair st = Col::all(ckpt_step(e));
+#pragma unroll
+            for (int i = 0; i < Col::N; ++i) xm.e[i] = vfma(xm.e[i], st, np);
+        } else {
+            float f[VEC];
+            unpack<T>(v, f);
+            xm.set(f);
+#pragma unroll
+            for (int i = 0; i < Col::N; ++i) xm.e[i] = vadd(xm.e[i], np);
+        }
+    };
+    // use(x - pivot, grad_out) for each of this thread's vectors
+    auto each = [&](Pair np, auto use) {
+        int left = mine;
+        for (int c = 0; c < w.chunks; ++c, left -= kRounds) {
+            ring.wait_full();
+            const unsigned char *p = shared + ring.stage * kChunkBytes;
+            uint4 d[kRounds];
+            X v[kRounds];
+            uint8_t e[kRounds];
+#pragma unroll
+            for (int k = 0; k < kRounds; ++k) {
+                d[k] = reinterpret_cast<const uint4 *>(p)[place_in + k * round];
+                v[k] = reinterpret_cast<const X *>(p + kBytes)[place_in + k * round];
+                e[k] = scale[k];
+            }
+            ring.release();
+            load_scales(left - kRounds);
+            auto vector = [&](int k) {
+                float f[VEC];
+                Col xm, dc;
+                unpack<T>(d[k], f);
+                dc.set(f);
+                shifted(v[k], e[k], np, xm);
+                use(xm, dc);
+            };
+            if (left >= kRounds) {
+#pragma unroll
+                for (int k = 0; k < kRounds; ++k) vector(k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kRounds; ++k)
+                    if (k < left) vector(k);
+            }
+        }
     };
 
     // z = (x - pivot) p + q as in the forward pass
     auto coefficients = [&](int slice, int64_t image, bool second) {
-        __syncthreads();                              // the arrays may still be read by the pass before
+        block_sync();                              // the arrays may still be read by the pass before
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
-            const int channel = slice * w.ncols + c, head = channel - c % VEC;
-            const int64_t st = image * a.groups + channel / a.width;
-            const float mean = a.b.mean[st], rs = a.b.rstd[st], pivot = a.b.mean[image * a.groups + head / a.width];
+            const int channel = slice * w.ncols + c;
+            const int64_t group0 = image * a.groups + slice * w.slice_groups;
+            const int64_t st = group0 + group_of[c];
+            const float mean = a.b.mean[st], rs = a.b.rstd[st], pivot = a.b.mean[group0 + group_of[c - c % VEC]];
             const float scale = a.b.gamma[channel] * rs;
             cp[c] = scale;
             cq[c] = fmaf(pivot - mean, scale, a.b.beta[channel]);
             pivots[c] = -pivot;
             if (second) {
-                const float2 s = stat[c / a.width];
+                const float2 s = stat[group_of[c]];
                 c1[c] = -rs * rs * s.y;
                 c0[c] = fmaf(pivot - mean, c1[c], -rs * s.x);
             }
         }
-        __syncthreads();
+        block_sync();
     };
 
     auto sums = [&](int slice, int64_t image) {
+        first_scales(slice, image);
         coefficients(slice, image, false);
         Col s0, s1;
 #pragma unroll
@@ -573,22 +676,14 @@ cl_team_backward_kernel(const Args a) {
             column_load<VEC>(cp + col, cs);
             column_load<VEC>(cq + col, ch);
             const Pair np = Col::all(pivots[col]);
-            int64_t at = (image * a.hw + w.first + w.row) * blocks_row + (slice * w.ncols + w.col * VEC) / kCkptBlock;
-            for (int r = 0; r < chunks * kChunkGrad; r += kChunkGrad, at += static_cast<int64_t>(kChunkGrad) * a.p.rows * blocks_row) {
-                Col xc[kChunkGrad], dc[kChunkGrad];
-                take_chunk(xc, dc, at);
+            each(np, [&](const Col &xm, const Col &dc) {
 #pragma unroll
-                for (int k = 0; k < kChunkGrad; ++k)
-                    if (r + k < w.mine) {
-#pragma unroll
-                        for (int i = 0; i < Col::N; ++i) {
-                            const Pair xm = vadd(xc[k].e[i], np);
-                            const Pair dz = act_grad<ACT>(dc[k].e[i], vfma(xm, cs.e[i], ch.e[i]), one, minus_one);
-                            s0.e[i] = vadd(s0.e[i], dz);
-                            s1.e[i] = vfma(dz, xm, s1.e[i]);
-                        }
-                    }
-            }
+                for (int i = 0; i < Col::N; ++i) {
+                    const Pair dz = act_grad<ACT>(dc.e[i], vfma(xm.e[i], cs.e[i], ch.e[i]), one, minus_one);
+                    s0.e[i] = vadd(s0.e[i], dz);
+                    s1.e[i] = vfma(dz, xm.e[i], s1.e[i]);
+                }
+            });
         }
         if (w.active) {
             float *to = buf + w.row * 2 * w.ncols + w.col * VEC;
@@ -598,14 +693,14 @@ cl_team_backward_kernel(const Args a) {
         sum_rows(buf, a.p.rows, 2 * w.ncols);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
-            const int64_t st = group0 + c / a.width;
+            const int64_t st = group0 + group_of[c];
             // from sums around the pivot to sums of dz xhat
             const float t = fmaf(-pivots[c] - a.b.mean[st], buf[c], buf[w.ncols + c]) * a.b.rstd[st];
             buf[w.ncols + c] = t;
             total[c] += buf[c];
             total[w.ncols + c] += t;
         }
-        __syncthreads();
+        block_sync();
         for (int g0 = 0; g0 < w.slice_groups; g0 += seg.per_block) {
             const int g = g0 + seg.mine;
             const int end = g < w.slice_groups ? (g + 1) * a.width : 0;
@@ -623,17 +718,20 @@ cl_team_backward_kernel(const Args a) {
     };
 
     auto apply = [&](int slice, int64_t image) {
+        first_scales(slice, image);
         wait_all(a, image * a.p.slices + slice);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float inv = 1.0f / (static_cast<float>(a.hw) * static_cast<float>(a.width));
         for (int g = warp; g < w.slice_groups; g += kWarps) {
-            float2 v[kMergeLoads];
-            load_partials(a, group0 + g, lane, v);
             float t1 = 0.f, t2 = 0.f;
+            for (int first = 0; first < a.p.members; first += 32 * kMergeLoads) {
+                float2 v[kMergeLoads];
+                load_partials(a, group0 + g, first + lane, v);
 #pragma unroll
-            for (int k = 0; k < kMergeLoads; ++k) {
-                t1 += v[k].x;
-                t2 += v[k].y;
+                for (int k = 0; k < kMergeLoads; ++k) {
+                    t1 += v[k].x;
+                    t2 += v[k].y;
+                }
             }
             t1 = warp_sum(t1);
             t2 = warp_sum(t2);
@@ -647,44 +745,35 @@ cl_team_backward_kernel(const Args a) {
         column_load<VEC>(c0 + col, k0);
         column_load<VEC>(c1 + col, k1);
         const Pair np = Col::all(pivots[col]);
-        int64_t at = (image * a.hw + w.first + w.row) * blocks_row + (slice * w.ncols + w.col * VEC) / kCkptBlock;
         T *o = dx + image * a.hw * a.channels + slice * w.ncols + mine0;
-        for (int r = 0; r < chunks * kChunkGrad; r += kChunkGrad, o += kChunkGrad * step,
-                 at += static_cast<int64_t>(kChunkGrad) * a.p.rows * blocks_row) {
-            Col xc[kChunkGrad], dc[kChunkGrad];
-            take_chunk(xc, dc, at);
+        each(np, [&](const Col &xm, Col &dc) {
 #pragma unroll
-            for (int k = 0; k < kChunkGrad; ++k)
-                if (r + k < w.mine) {
-#pragma unroll
-                    for (int i = 0; i < Col::N; ++i) {
-                        const Pair xm = vadd(xc[k].e[i], np);
-                        const Pair dz = act_grad<ACT>(dc[k].e[i], vfma(xm, cs.e[i], ch.e[i]), one, minus_one);
-                        dc[k].e[i] = vfma(dz, cs.e[i], vfma(xm, k1.e[i], k0.e[i]));
-                    }
-                    float f[VEC];
-                    dc[k].get(f);
-                    st_stream(o + k * step, pack<T>(f));
-                }
-        }
+            for (int i = 0; i < Col::N; ++i) {
+                const Pair dz = act_grad<ACT>(dc.e[i], vfma(xm.e[i], cs.e[i], ch.e[i]), one, minus_one);
+                dc.e[i] = vfma(dz, cs.e[i], vfma(xm.e[i], k1.e[i], k0.e[i]));
+            }
+            float f[VEC];
+            dc.get(f);
+            st_stream(o, pack<T>(f));
+            o += step;
+        });
     };
 
-    for (int k = 0; k < kStagesGrad; ++k) load_chunk();
-    for (int p = 0; p < items.passes(); ++p) {
-        bool second;
-        const int k = items.item(p, &second), slice = items.slice(k);
-        if (second) {
-            apply(slice, items.image(k));
+    int summed = -1;                                  // the slice that `total` belongs to
+    while (passes.next(a, w)) {
+        const int slice = passes.now.slice;
+        if (passes.second) {
+            apply(slice, passes.now.image);
             continue;
         }
-        const bool first = k % items.images == 0, last = k % items.images == items.images - 1;
-        if (first) {
-            __syncthreads();
+        if (slice != summed) {
+            block_sync();
             for (int c = threadIdx.x; c < 2 * w.ncols; c += kThreads) total[c] = 0.f;
+            summed = slice;
         }
-        sums(slice, items.image(k));
-        if (last) {
-            __syncthreads();
+        sums(slice, passes.now.image);
+        if (passes.now.image + a.p.image_teams >= static_cast<int>(a.batch)) {                             // the slice's last image
+            block_sync();
             const int64_t entry = static_cast<int64_t>(w.image_team) * a.p.members + w.member;
             float2 *to = a.channel_sums + (static_cast<int64_t>(slice) * a.p.image_teams * a.p.members + entry) * w.ncols;
             for (int c = threadIdx.x; c < w.ncols; c += kThreads) to[c] = make_float2(total[c], total[w.ncols + c]);
@@ -745,8 +834,10 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
     a.channels = s.channels;
     a.groups = s.groups;
     a.width = static_cast<int>(s.channels / s.groups);
-    a.share = static_cast<int>(s.hw / p.members);
-    a.rest = static_cast<int>(s.hw % p.members);
+    a.chunk_rows = p.rows * kRounds;
+    const int64_t chunks = (s.hw + a.chunk_rows - 1) / a.chunk_rows;
+    a.share = static_cast<int>(chunks / p.members);
+    a.rest = static_cast<int>(chunks % p.members);
     a.eps = s.eps;
     a.arrived = reinterpret_cast<unsigned int *>(base);
     a.partial = reinterpret_cast<float2 *>(base + l.partial);
@@ -754,21 +845,55 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
     return a;
 }
 
-size_t shared_bytes(const GnClTeamPlan &p, bool backward) {
+size_t shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt) {
     const size_t ncols = static_cast<size_t>(p.cols) * p.vec;
-    const size_t ring = backward ? static_cast<size_t>(kChunkGrad) * kStagesGrad * 2 : static_cast<size_t>(kChunk) * kStages;
-    return ring * kThreads * 16 + (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 9 : 5) * ncols) * sizeof(float);
+    const size_t vector = !backward ? 16 : ckpt ? 16 + p.vec : 32;
+    return static_cast<size_t>(backward ? kStagesGrad : kStages) * kRounds * kThreads * vector +
+           (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 10 : 6) * ncols) * sizeof(float);
 }
 
-cudaError_t launch(void (*kernel)(Args), const Args &a, bool backward, cudaStream_t stream) {
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, looked up once (the library does not link the driver).
+EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// [rows, row_bytes] in 8-byte units; boxes of box_bytes by box_rows.  row_bytes and box_bytes are multiples
+// of 16, base 16-byte aligned.
+cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t row_bytes, int box_bytes, int box_rows) {
+    const EncodeFn fn = encoder();
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes / 8), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / 8), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t steps[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<void *>(base), dims, strides, box, steps,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// A cooperative launch: the blocks of a team wait for one another, so either all of them run or none.
+template <typename... Maps>
+cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
     cudaError_t err = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(a.batch) * a.p.slices * sizeof(unsigned int), stream);
     if (err != cudaSuccess) return err;
-    const size_t smem = shared_bytes(a.p, backward);
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.p.slice_teams * a.p.image_teams * a.p.members));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kBlock);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -776,25 +901,37 @@ cudaError_t launch(void (*kernel)(Args), const Args &a, bool backward, cudaStrea
     attr[0].val.cooperative = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.p.members > 1 ? 1 : 0;
-    err = cudaLaunchKernelEx(&cfg, kernel, a);
+    err = cudaLaunchKernelEx(&cfg, kernel, a, maps...);
     if (err == cudaSuccess) g_launches.fetch_add(1);
     return err;
 }
 
 template <typename T> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+    CUtensorMap x;
+    const cudaError_t err = make_map(&x, a.f.in, s.batch * s.hw, s.channels * sizeof(T), a.p.cols * 16, a.chunk_rows);
+    if (err != cudaSuccess) return err;
+    const size_t smem = shared_bytes(a.p, false, false);
     if (s.act == kActSilu)
-        return a.f.codes ? launch(cl_team_forward_kernel<T, kActSilu, true>, a, false, stream)
-                         : launch(cl_team_forward_kernel<T, kActSilu, false>, a, false, stream);
-    return a.f.codes ? launch(cl_team_forward_kernel<T, kActNone, true>, a, false, stream)
-                     : launch(cl_team_forward_kernel<T, kActNone, false>, a, false, stream);
+        return a.f.codes ? launch(cl_team_forward_kernel<T, kActSilu, true>, a, smem, stream, x)
+                         : launch(cl_team_forward_kernel<T, kActSilu, false>, a, smem, stream, x);
+    return a.f.codes ? launch(cl_team_forward_kernel<T, kActNone, true>, a, smem, stream, x)
+                     : launch(cl_team_forward_kernel<T, kActNone, false>, a, smem, stream, x);
 }
 
 template <typename T> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+    const int64_t rows = s.batch * s.hw, row_bytes = s.channels * sizeof(T);
+    CUtensorMap x, dy;
+    cudaError_t err = make_map(&dy, a.b.grad_out, rows, row_bytes, a.p.cols * 16, a.chunk_rows);
+    if (err == cudaSuccess)
+        err = a.b.codes ? make_map(&x, a.b.codes, rows, s.channels, a.p.cols * a.p.vec, a.chunk_rows)
+                        : make_map(&x, a.b.in, rows, row_bytes, a.p.cols * 16, a.chunk_rows);
+    if (err != cudaSuccess) return err;
+    const size_t smem = shared_bytes(a.p, true, a.b.codes != nullptr);
     if (s.act == kActSilu)
-        return a.b.codes ? launch(cl_team_backward_kernel<T, kActSilu, true>, a, true, stream)
-                         : launch(cl_team_backward_kernel<T, kActSilu, false>, a, true, stream);
-    return a.b.codes ? launch(cl_team_backward_kernel<T, kActNone, true>, a, true, stream)
-                     : launch(cl_team_backward_kernel<T, kActNone, false>, a, true, stream);
+        return a.b.codes ? launch(cl_team_backward_kernel<T, kActSilu, true>, a, smem, stream, x, dy)
+                         : launch(cl_team_backward_kernel<T, kActSilu, false>, a, smem, stream, x, dy);
+    return a.b.codes ? launch(cl_team_backward_kernel<T, kActNone, true>, a, smem, stream, x, dy)
+                     : launch(cl_team_backward_kernel<T, kActNone, false>, a, smem, stream, x, dy);
 }
 
 }  // namespace
@@ -804,9 +941,12 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     const int64_t esize = s.dtype == kF32 ? 4 : 2;
     p->vec = static_cast<int>(16 / esize);
     if (s.channels % p->vec != 0 || (pack && s.channels % kCkptBlock != 0)) return false;
-    // the narrowest slice, in columns: whole groups, whole vectors and, when it is packed, whole blocks
+    if (s.batch * s.hw >= (1ll << 31)) return false;                                  // box coordinates
+    // the narrowest slice, in columns: whole groups, whole vectors, and of a checkpoint whole blocks
+    // (written) or 16 bytes of codes (read)
     int64_t grain = std::lcm(width, static_cast<int64_t>(p->vec));
     if (pack) grain = std::lcm(grain, static_cast<int64_t>(kCkptBlock));
+    if (ckpt) grain = std::lcm(grain, static_cast<int64_t>(16));
     if (grain > s.channels || s.channels % grain != 0) return false;
     const int64_t grains = s.channels / grain;
     grain /= p->vec;
@@ -830,10 +970,10 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     }
     p->slices = static_cast<int>(best);
     p->cols = static_cast<int>(grains / best * grain);
-    p->rows = kThreads / p->cols;
+    p->rows = std::min(kThreads / p->cols, 256 / kRounds);                             // a box has at most 256 rows
     // what an SM holds at once: 228 KB of shared memory, 1 KB of it reserved per block
-    const int64_t fit = 228 * 1024 / (static_cast<int64_t>(shared_bytes(*p, backward)) + 1024);
-    const int64_t blocks = static_cast<int64_t>(sm_count()) * std::min<int64_t>(fit, backward ? kBlocksPerSmGrad : kBlocksPerSm);
+    const int64_t fit = 228 * 1024 / (static_cast<int64_t>(shared_bytes(*p, backward, ckpt)) + 1024);
+    const int64_t blocks = static_cast<int64_t>(sm_count()) * std::min<int64_t>(fit, kBlocksPerSm);
     if (least > 1) {
         p->slice_teams = 1;
         p->image_teams = 1;
@@ -847,8 +987,9 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
         if (p->slice_teams > blocks) p->slice_teams = static_cast<int>(blocks);
     }
     int64_t m = std::max<int64_t>(1, blocks / (static_cast<int64_t>(p->slice_teams) * p->image_teams));
-    m = std::min(m, std::max<int64_t>(1, s.hw / (p->rows * 2)));                      // at least two pixels per thread
-    p->members = static_cast<int>(std::min<int64_t>(m, kMaxMembers));
+    m = std::min(m, (s.hw + p->rows * kRounds - 1) / (p->rows * kRounds));            // a chunk each at least
+    p->members = static_cast<int>(m);
+    p->lag = m > 1 ? 1 : 0;
     return true;
 }
 
