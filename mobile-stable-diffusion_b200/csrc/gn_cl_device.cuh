@@ -17,6 +17,8 @@
 #include "ckpt_device.cuh"
 #include "kernels.h"
 
+#include <type_traits>
+
 namespace sdfl {
 
 namespace {
@@ -140,11 +142,57 @@ __device__ __forceinline__ void codes4(uint32_t w, Pair &lo, Pair &hi) {
     lo = vadd(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540u)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541u))), offset);
     hi = vadd(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7542u)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7543u))), offset);
 }
-__device__ __forceinline__ void code_column(const uint2 &w, Column<8> &c) {
-    codes4(w.x, c.e[0], c.e[1]);
-    codes4(w.y, c.e[2], c.e[3]);
+
+// Half h of a column (4 elements, two pairs) out of a vector of T, or out of its codes.
+template <typename T> __device__ __forceinline__ void half_column(const uint4 &v, int h, Pair (&e)[2]) {
+    if constexpr (sizeof(T) == 4) {
+        e[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y));
+        e[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
+    } else {
+        const uint32_t w[2] = {h ? v.z : v.x, h ? v.w : v.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                e[i] = pair(f.x, f.y);
+            } else {
+                e[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            }
+        }
+    }
 }
-__device__ __forceinline__ void code_column(uint32_t w, Column<4> &c) { codes4(w, c.e[0], c.e[1]); }
+__device__ __forceinline__ void half_codes(const uint2 &w, int h, Pair (&e)[2]) { codes4(h ? w.y : w.x, e[0], e[1]); }
+__device__ __forceinline__ void half_codes(uint32_t w, int, Pair (&e)[2]) { codes4(w, e[0], e[1]); }
+
+// Two pairs back to storage: a half of a 16-bit vector, all of an fp32 one.
+template <typename T> __device__ __forceinline__ void half_pack(uint4 &v, int h, const Pair (&e)[2]) {
+    float f[4];
+    split(e[0], f[0], f[1]);
+    split(e[1], f[2], f[3]);
+    if constexpr (sizeof(T) == 4) {
+        v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    } else {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&p);
+            } else {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&p);
+            }
+        }
+        (h ? v.z : v.x) = w[0];
+        (h ? v.w : v.y) = w[1];
+    }
+}
+// Four floats of shared memory as two pairs.
+__device__ __forceinline__ void quad_load(const float *from, Pair (&e)[2]) {
+    const float4 v = *reinterpret_cast<const float4 *>(from);
+    e[0] = pair(v.x, v.y);
+    e[1] = pair(v.z, v.w);
+}
 
 // VEC floats of shared memory, 16 bytes at a time (rows of a thread's column are 16-byte aligned).
 template <int VEC> __device__ __forceinline__ void shared_store(float *to, const float (&f)[VEC]) {
@@ -175,26 +223,39 @@ template <int VEC> __device__ __forceinline__ void column_store(float *to, const
     shared_store<VEC>(to, f);
 }
 
-// sigmoid with the SFU exp2 and reciprocal (relative error about 2^-21).  A pair shares one reciprocal,
-// 1 / (a b), from which 1 / a = b / (a b): three SFU operations per pair instead of four (they run at
-// an eighth of the issue rate and are the next limit after the issue slots).  The exponent is held
-// at 60 so that a b stays finite; below z = -41 the sigmoid is then 2^-60 instead of less than that.
-__device__ __forceinline__ float sigmoid_fast(float z) {
-    return rcp_approx(1.0f + ex2_approx(fminf(-1.4426950408889634f * z, 60.0f)));
+// s = sigmoid(z) and, where asked for, w = 1 - s, from t = exp(-z): s = 1 / (1 + t), w = t s, with the SFU
+// exp2 and reciprocal (relative error about 2^-21).  A pair shares one reciprocal, 1 / (a b), from which
+// 1 / a = b / (a b): three SFU operations per pair instead of four (they run at an eighth of the
+// issue rate).  The exponent is held at 60 so that a b stays finite; below z = -41 the sigmoid is then
+// 2^-60 instead of less than that.
+__device__ __forceinline__ void sigmoid_fast(float z, float &s, float &w) {
+    const float t = ex2_approx(fminf(-1.4426950408889634f * z, 60.0f));
+    s = rcp_approx(1.0f + t);
+    w = t * s;
 }
-__device__ __forceinline__ Pair sigmoid_fast(Pair z) {
+__device__ __forceinline__ void sigmoid_fast(Pair z, Pair &s, Pair &w) {
     float lo, hi, a, b;
     split(vmul(z, pair(-1.4426950408889634f, -1.4426950408889634f)), lo, hi);
-    split(vadd(pair(ex2_approx(fminf(lo, 60.0f)), ex2_approx(fminf(hi, 60.0f))), pair(1.0f, 1.0f)), a, b);
+    const Pair t = pair(ex2_approx(fminf(lo, 60.0f)), ex2_approx(fminf(hi, 60.0f)));
+    split(vadd(t, pair(1.0f, 1.0f)), a, b);
     const float r = rcp_approx(a * b);
-    return pair(b * r, a * r);
+    s = pair(b * r, a * r);
+    w = vmul(t, s);
 }
 
-// dy act'(z), silu'(z) = s (1 + z (1 - s)) with s = sigmoid(z).
-template <int ACT, typename E> __device__ __forceinline__ E act_grad(E dy, E z, E one, E minus_one) {
+template <int ACT, typename E> __device__ __forceinline__ E act_value(E z) {
+    if (ACT != kActSilu) return z;
+    E s, w;
+    sigmoid_fast(z, s, w);
+    return vmul(z, s);
+}
+
+// dy act'(z), silu'(z) = s (1 + z (1 - s)).
+template <int ACT, typename E> __device__ __forceinline__ E act_grad(E dy, E z, E one) {
     if (ACT != kActSilu) return dy;
-    const E s = sigmoid_fast(z);
-    return vmul(vmul(dy, s), vfma(z, vfma(s, minus_one, one), one));
+    E s, w;
+    sigmoid_fast(z, s, w);
+    return vmul(vmul(dy, s), vfma(z, w, one));
 }
 
 }  // namespace

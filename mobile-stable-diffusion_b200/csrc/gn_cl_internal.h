@@ -19,7 +19,7 @@ struct GnClTeamPlan {
     int slice_teams;       // teams side by side on the slices of an image
     int image_teams;       // teams side by side on images
     int members;           // thread blocks per team
-    int lag;               // teams that run S of the next item before A of the current: 0 none, 1 all, 2 every other one
+    int stagger;           // odd teams start behind the even ones' first pass
 };
 // false: no plan for this shape.  pack: the forward pass also writes a checkpoint; ckpt: the
 // backward pass reads one.

@@ -85,7 +85,7 @@ template <int VEC, int ACT> struct Normalise {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float z = fmaf(f[i] - pivot, p[i], q[i]);
-            f[i] = ACT == kActSilu ? z * sigmoid_fast(z) : z;
+            f[i] = act_value<ACT>(z);
         }
     }
 };
@@ -246,7 +246,7 @@ cl_grad_sums_kernel(GnClBackward a, float2 *partial, Geometry g, int64_t hw, int
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float xm = x[i] - mean[i];
-                const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f, -1.0f);
+                const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f);
                 s0[i] += dz;
                 s1[i] = fmaf(dz, xm, s1[i]);
             }
@@ -348,7 +348,7 @@ cl_grad_input_kernel(GnClBackward a, const float2 *__restrict__ group_sums, Geom
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float xm = x[i] - mean[i];
-            const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f, -1.0f);
+            const float dz = act_grad<ACT>(d[i], fmaf(xm, p[i], q[i]), 1.0f);
             d[i] = fmaf(dz, p[i], -fmaf(xm, c1[i], c0[i]));
         }
         raw_store<T, VEC>(dx + row * channels + w.channel, raw_pack<T, VEC>(d));

@@ -7,11 +7,15 @@
 // the second read inside L2.
 //
 // Split.  An item is a slice of an image's channels (whole groups and whole vectors, a 128-byte row or
-// more where the sizes allow it) over all its pixels.  A team of M thread blocks works on one item at a
-// time, each block on its own range of pixels: pass S reads and sums, the blocks' sums are exchanged, pass
-// A reads again and writes.  The bytes of all teams' open items stay below kInFlight, so that the
-// second read comes from L2 whatever the tensor's size.  A team with more than one item runs S of the
-// next item between S and A of the current one, which hides the exchange.
+// more where the sizes allow it) over all its pixels.  A team of M thread blocks goes through its items
+// together, each block on its own range of pixels: pass S reads and sums, the blocks' sums are exchanged,
+// pass A reads again and writes.  The bytes of all teams' open items stay below kInFlight, so that the
+// second read comes from L2 whatever the tensor's size.  An SM holds blocks of two teams, the odd ones
+// started behind the even ones' first pass S, so that one team's reading, which waits for HBM, and its
+// exchange run beside the other's writing, which computes.
+// (Alternating the chunks of S of one item with those of A of another in the same block was tried and is
+// 15 % slower: three items per team are open then, so they are smaller, and what a block spends per
+// item -- about 5 us for adding up and exchanging -- is paid more often.)
 //
 // Loads.  A producer warp keeps a ring of chunks filled by tiled bulk copies (a chunk is kRounds rows per
 // consumer thread, the box of a 2-D tensor map over [batch * hw, channels]); the consumer warps wait on
@@ -20,10 +24,13 @@
 // pass are already under way.  The copies cost the consumers no issue slots, and those are what the
 // gradient runs short of first (per-thread cp.async into the same ring: 12 more instructions per vector).
 //
-// Exchange.  A block writes its sums per group to the workspace and counts itself in; before pass A every
-// block polls the count and merges all of the team's sums itself, in block order (the same bits on
-// every run).  Every block of the grid is resident (cooperative launch), and every wait is
-// bounded: on time-out the status word is raised and the launch finishes with an invalid result.
+// Exchange.  A block writes its sums per group to the workspace and counts itself in (the counters are
+// zeroed by a small kernel in front); before pass A one thread of a block polls the count, then
+// the block merges all of the team's sums itself, in block order (the same bits on every run).  Every
+// block of the grid is resident (cooperative launch), and every wait is bounded: on time-out the
+// status word is raised and the launch finishes with an invalid result.
+// (Sums that carry their own "written" mark, polled by all warps, save the fence and the counter but
+// were 10 % slower: the polling takes issue slots and L2 bandwidth from the blocks that still compute.)
 //
 // Weight gradients: a block adds up its channels' sums over the images of its slice in shared memory and
 // writes them once per slice; cl_param_sum_kernel adds the blocks' rows.
@@ -44,11 +51,14 @@ constexpr int kThreads = 256;                      // consumers
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = kThreads + 32;              // and the producer warp
 constexpr int kBlocksPerSm = 2;
-constexpr int kRounds = 2;                         // rows per thread and chunk
-constexpr int kStages = 6, kStagesGrad = 5;        // chunks of the ring: 8 KB per tensor each
+// Rows per thread and chunk, and chunks of the ring.
+constexpr int kRounds = 4, kStages = 5;            // 16 KB chunks
+constexpr int kRoundsGrad = 4, kStagesGrad = 3;    // 16 KB of grad_out and 16, 8 or 4 KB of x or its codes
 constexpr int kMaxCols = kThreads / 2;             // columns of a slice: a box row of 2 KB
 constexpr int kMergeLoads = 5;                     // a team of up to 160 blocks in one round
 constexpr int64_t kInFlight = 64ll << 20;
+constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
+constexpr int kSlotWords = 1024 + kMaxTeamsOfSm;
 
 __device__ unsigned int g_cl_status;               // bit 0: a bounded wait ran out
 
@@ -61,13 +71,14 @@ struct Args {                    // one struct for both directions
     int chunk_rows;              // pixels per chunk
     int share, rest;             // chunks of an image / members, % members
     float eps;
-    unsigned int *arrived;       // [items]
+    unsigned int *arrived;       // [items], then kSlotWords for the placement of blocks
+    long long items;
     float2 *partial;             // [batch * groups][members]
     float2 *channel_sums;        // [slice][image_teams * members][slice channels]
 };
 
 struct Place {
-    int member, slice_team, image_team, col, row, ncols, slice_groups;
+    int team, member, slice_team, image_team, col, row, ncols, slice_groups;
     int first, chunks, pixels;   // this block's pixels of every item: [first, first + pixels)
     bool active;
 };
@@ -81,12 +92,31 @@ __device__ __forceinline__ int member_pixels(const Args &a, int member) {
     return min(static_cast<int>(a.hw) - first, (a.share + (member < a.rest ? 1 : 0)) * a.chunk_rows);
 }
 
+// Two teams that run out of step must share every SM evenly: two blocks of one team on an SM would do their
+// computing at the same time and keep the rest of the team waiting (the hardware puts blocks i and
+// i + #SMs together on most SMs only; 23 instead of 14 us for pass A on the others).  So a block takes its
+// number from its SM: the SM's k-th block is a member of team k.
+__device__ __forceinline__ int block_number(const Args &a) {
+    if (!a.p.stagger) return blockIdx.x;
+    __shared__ int number;
+    if (threadIdx.x == 0) {
+        unsigned int sm;
+        asm volatile("mov.u32 %0, %smid;" : "=r"(sm));
+        unsigned int *slots = a.arrived + a.items;
+        const unsigned int slot = atomicAdd(slots + kMaxTeamsOfSm + sm % (kSlotWords - kMaxTeamsOfSm), 1u) % kMaxTeamsOfSm;
+        number = static_cast<int>(slot * a.p.members + atomicAdd(slots + slot, 1u) % a.p.members);
+    }
+    __syncthreads();
+    return number;
+}
+
 __device__ __forceinline__ Place place(const Args &a) {
     Place w;
-    const int team = blockIdx.x / a.p.members;
-    w.member = blockIdx.x - team * a.p.members;
-    w.slice_team = team % a.p.slice_teams;
-    w.image_team = team / a.p.slice_teams;
+    const int block = block_number(a);
+    w.team = block / a.p.members;
+    w.member = block - w.team * a.p.members;
+    w.slice_team = w.team % a.p.slice_teams;
+    w.image_team = w.team / a.p.slice_teams;
     w.row = threadIdx.x / a.p.cols;
     w.col = threadIdx.x - w.row * a.p.cols;
     w.active = w.row < a.p.rows;
@@ -110,32 +140,21 @@ struct Cursor {
     }
 };
 
-// The order of a team's passes: S0 A0 S1 A1 ..., or with a lag S0, S1 A0, S2 A1, ... and the last A.
+// A team's passes: S and A of an item, then the next item.
 struct Passes {
-    Cursor s, a, now;
-    bool lag, sum_next, second;
-    __device__ __forceinline__ Passes(const Args &args, const Place &w) {
-        s = a = now = Cursor{w.slice_team, w.image_team};
-        lag = args.p.lag == 1 || (args.p.lag == 2 && ((w.image_team * args.p.slice_teams + w.slice_team) & 1));
-        sum_next = true;
-        second = false;
+    Cursor now;
+    bool second;
+    __device__ __forceinline__ explicit Passes(const Place &w) : now{w.slice_team, w.image_team}, second(true) {
+        now.image -= 1;                               // nothing yet
     }
     // false: none left
-    __device__ __forceinline__ bool next(const Args &args, const Place &w) {
-        const bool more = s.slice < args.p.slices;
-        if (!more && a.slice >= args.p.slices) return false;
-        if (more && sum_next) {
-            second = false;
-            now = s;
-            s.next(args, w);
-            sum_next = lag;                           // once: one S ahead from here on
-            lag = false;
-        } else {
-            second = sum_next = true;
-            now = a;
-            a.next(args, w);
+    __device__ __forceinline__ bool next(const Args &a, const Place &w) {
+        second = !second;
+        if (!second) {
+            if (now.image < w.image_team) now.image = w.image_team;
+            else now.next(a, w);
         }
-        return true;
+        return now.slice < a.p.slices;
     }
 };
 
@@ -187,6 +206,7 @@ template <int STAGES> struct Ring {
 
 __device__ __forceinline__ void block_sync() { consumer_sync(kThreads); }       // the consumer warps
 
+// ---- exchange ---------------------------------------------------------------------------------------
 // Counts the block in on an item; its sums were written (by any thread) before.
 __device__ __forceinline__ void arrive(const Args &a, int64_t item) {
     block_sync();
@@ -196,24 +216,27 @@ __device__ __forceinline__ void arrive(const Args &a, int64_t item) {
     }
 }
 
+__device__ __forceinline__ void wait_count(const Args &a, int64_t item, unsigned int count, unsigned int sleep) {
+    const long long t0 = clock64();
+    for (;;) {
+        unsigned int v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(a.arrived + item) : "memory");
+        if (v >= count) break;
+        if (clock64() - t0 > kWaitCycles) {
+            atomicOr(&g_cl_status, 1u);
+            break;
+        }
+        if (sleep) __nanosleep(sleep);
+    }
+}
+
 // Waits until all of the team's blocks have counted themselves in.
 __device__ __forceinline__ void wait_all(const Args &a, int64_t item) {
-    if (threadIdx.x == 0) {
-        unsigned int v;
-        const long long t0 = clock64();
-        for (;;) {
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(a.arrived + item) : "memory");
-            if (v >= static_cast<unsigned>(a.p.members)) break;
-            if (clock64() - t0 > kWaitCycles) {
-                atomicOr(&g_cl_status, 1u);
-                break;
-            }
-        }
-    }
+    if (threadIdx.x == 0) wait_count(a, item, static_cast<unsigned>(a.p.members), 0);
     block_sync();
 }
 
-// One group's sums of all the team's blocks, kMergeLoads * 32 per round with every load in flight at once.
+// One group's sums of up to 32 * kMergeLoads blocks from `first` on, every load in flight at once.
 __device__ __forceinline__ void load_partials(const Args &a, int64_t group, int first, float2 (&v)[kMergeLoads]) {
     const float2 *q = a.partial + group * a.p.members + first;
 #pragma unroll
@@ -224,6 +247,14 @@ __device__ __forceinline__ void load_partials(const Args &a, int64_t group, int 
 }
 __device__ __forceinline__ float pixels_or_none(const Args &a, int member) {
     return member < a.p.members ? static_cast<float>(member_pixels(a, member)) : 0.f;
+}
+
+// Odd teams start when half of the blocks of the team before them are through their first pass S.
+__device__ __forceinline__ void stagger(const Args &a, int team) {
+    if (!a.p.stagger || !(team & 1)) return;
+    const int before = team - 1;
+    wait_count(a, static_cast<int64_t>(before / a.p.slice_teams) * a.p.slices + before % a.p.slice_teams,
+               static_cast<unsigned>((a.p.members + 1) / 2), 200);
 }
 
 // Groups of a slice are dealt to segments of L lanes, L the largest power of two up to the group's width.
@@ -298,7 +329,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (mean, rstd)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Passes passes(a, w);
+    Passes passes(w);
     Ring<kStages> ring;
     ring.init(bars);
     for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
@@ -306,6 +337,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
+            stagger(a, w.team);
             const uint64_t again = policy_evict_last(), done = policy_evict_first();
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols * sizeof(T));
             while (passes.next(a, w)) {
@@ -336,18 +368,13 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
         for (int c = 0; c < w.chunks; ++c, left -= kRounds) {
             ring.wait_full();
             const uint4 *p = mine_in + ring.stage * (kChunkBytes / 16);
-            uint4 v[kRounds];
-#pragma unroll
-            for (int k = 0; k < kRounds; ++k) v[k] = p[k * round];
-            ring.release();
             if (left >= kRounds) {
 #pragma unroll
-                for (int k = 0; k < kRounds; ++k) one(v[k]);
+                for (int k = 0; k < kRounds; ++k) one(p[k * round]);
             } else {
-#pragma unroll
-                for (int k = 0; k < kRounds; ++k)
-                    if (k < left) one(v[k]);
+                for (int k = 0; k < left; ++k) one(p[k * round]);
             }
+            ring.release();
         }
     };
 
@@ -485,24 +512,22 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             pivots[c] = -pivot;
         }
         block_sync();
-        Col cs, ch;
         const int col = w.active ? w.col * VEC : 0;
-        column_load<VEC>(cp + col, cs);
-        column_load<VEC>(cq + col, ch);
         const Pair np = Col::all(pivots[col]);
         T *o = y + image * a.hw * a.channels + slice * w.ncols + mine0;
         each([&](const uint4 &v) {
-            float f[VEC];
-            unpack<T>(v, f);
-            Col c;
-            c.set(f);
+            uint4 r;
 #pragma unroll
-            for (int i = 0; i < Col::N; ++i) {
-                const Pair z = vfma(vadd(c.e[i], np), cs.e[i], ch.e[i]);
-                c.e[i] = ACT == kActSilu ? vmul(z, sigmoid_fast(z)) : z;
+            for (int h = 0; h < VEC / 4; ++h) {
+                Pair e[2], p[2], q[2];
+                half_column<T>(v, h, e);
+                quad_load(cp + col + 4 * h, p);
+                quad_load(cq + col + 4 * h, q);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) e[i] = act_value<ACT>(vfma(vadd(e[i], np), p[i], q[i]));
+                half_pack<T>(r, h, e);
             }
-            c.get(f);
-            st_stream(o, pack<T>(f));
+            st_stream(o, r);
             o += step;
         });
     };
@@ -518,8 +543,8 @@ template <typename T, int ACT, bool CKPT>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy) {
     constexpr int VEC = VecOf<T>::N;
-    constexpr int kBytes = kRounds * kThreads * 16;                  // grad_out's part of a chunk
-    constexpr int kBytesX = CKPT ? kRounds * kThreads * VEC : kBytes;
+    constexpr int kBytes = kRoundsGrad * kThreads * 16;                  // grad_out's part of a chunk
+    constexpr int kBytesX = CKPT ? kRoundsGrad * kThreads * VEC : kBytes;
     constexpr int kChunkBytes = kBytes + kBytesX;
     using Col = Column<VEC>;
     using X = std::conditional_t<CKPT, typename CodeVec<VEC>::type, uint4>;
@@ -536,7 +561,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (s1, s2)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    Passes passes(a, w);
+    Passes passes(w);
     Ring<kStagesGrad> ring;
     ring.init(bars);
     for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
@@ -544,6 +569,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
+            stagger(a, w.team);
             const uint64_t again = policy_evict_last(), done = policy_evict_first();
             constexpr int kSizeX = CKPT ? 1 : sizeof(T);
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols) * (sizeof(T) + kSizeX);
@@ -567,7 +593,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     const Segments seg(a.width);
     const int64_t blocks_row = ckpt_blocks(a.channels), scale_step = a.p.rows * blocks_row;
     T *dx = static_cast<T *>(a.b.grad_in);
-    const Pair one = Col::all(1.0f), minus_one = Col::all(-1.0f);
+    const Pair one = Col::all(1.0f);
     const int64_t step = static_cast<int64_t>(a.p.rows) * a.channels;
     const int64_t mine0 = (w.first + w.row) * a.channels + w.col * VEC;
     // this thread's vectors within a chunk, and its rows of a pass
@@ -576,13 +602,13 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     const int mine = w.active ? (w.pixels - w.row + a.p.rows - 1) / a.p.rows : 0;
     // The scale bytes of a checkpoint (less than 16 bytes a row) are loaded into registers one chunk ahead.
     const uint8_t *scale_at = nullptr;
-    uint8_t scale[kRounds] = {};
+    uint8_t scale[kRoundsGrad] = {};
     auto load_scales = [&](int left) {
         if constexpr (CKPT) {
 #pragma unroll
-            for (int k = 0; k < kRounds; ++k)
+            for (int k = 0; k < kRoundsGrad; ++k)
                 if (k < left) scale[k] = scale_at[k * scale_step];
-            scale_at += kRounds * scale_step;
+            scale_at += kRoundsGrad * scale_step;
         }
     };
     auto first_scales = [&](int slice, int64_t image) {
@@ -592,56 +618,52 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             load_scales(mine);
         }
     };
-    // x - pivot
-    auto shifted = [&](const X &v, uint8_t e, Pair np, Col &xm) {
-        if constexpr (CKPT) {
-            code_column(v, xm);
-            const Pair st = Col::all(ckpt_step(e));
-#pragma unroll
-            for (int i = 0; i < Col::N; ++i) xm.e[i] = vfma(xm.e[i], st, np);
-        } else {
-            float f[VEC];
-            unpack<T>(v, f);
-            xm.set(f);
-#pragma unroll
-            for (int i = 0; i < Col::N; ++i) xm.e[i] = vadd(xm.e[i], np);
-        }
-    };
-    // use(x - pivot, grad_out) for each of this thread's vectors
-    auto each = [&](Pair np, auto use) {
+    // use(h, coefficients, x - pivot, grad_out, vector) for both halves of each of this thread's vectors, then
+    // done(vector).  The coefficients are read from shared memory where they are used: held in
+    // registers they would take a third of the warps away.
+    auto each = [&](Pair np, auto coefficient, auto use, auto done) {
         int left = mine;
-        for (int c = 0; c < w.chunks; ++c, left -= kRounds) {
+        for (int c = 0; c < w.chunks; ++c, left -= kRoundsGrad) {
             ring.wait_full();
             const unsigned char *p = shared + ring.stage * kChunkBytes;
-            uint4 d[kRounds];
-            X v[kRounds];
-            uint8_t e[kRounds];
+            uint8_t e[kRoundsGrad];
 #pragma unroll
-            for (int k = 0; k < kRounds; ++k) {
-                d[k] = reinterpret_cast<const uint4 *>(p)[place_in + k * round];
-                v[k] = reinterpret_cast<const X *>(p + kBytes)[place_in + k * round];
-                e[k] = scale[k];
-            }
-            ring.release();
-            load_scales(left - kRounds);
-            auto vector = [&](int k) {
-                float f[VEC];
-                Col xm, dc;
-                unpack<T>(d[k], f);
-                dc.set(f);
-                shifted(v[k], e[k], np, xm);
-                use(xm, dc);
+            for (int k = 0; k < kRoundsGrad; ++k) e[k] = scale[k];
+            load_scales(left - kRoundsGrad);
+            auto vector = [&](int k, uint8_t ek) {
+                uint4 d = reinterpret_cast<const uint4 *>(p)[place_in + k * round];
+                const X v = reinterpret_cast<const X *>(p + kBytes)[place_in + k * round];
+#pragma unroll
+                for (int h = 0; h < VEC / 4; ++h) {
+                    const auto coef = coefficient(h);
+                    Pair xm[2], g[2];
+                    half_column<T>(d, h, g);
+                    if constexpr (CKPT) {
+                        half_codes(v, h, xm);
+                        const Pair st = Col::all(ckpt_step(ek));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) xm[i] = vfma(xm[i], st, np);
+                    } else {
+                        half_column<T>(v, h, xm);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) xm[i] = vadd(xm[i], np);
+                    }
+                    use(h, coef, xm, g, d);
+                }
+                done(d);
             };
-            if (left >= kRounds) {
+            if (left >= kRoundsGrad) {
 #pragma unroll
-                for (int k = 0; k < kRounds; ++k) vector(k);
+                for (int k = 0; k < kRoundsGrad; ++k) vector(k, e[k]);
             } else {
 #pragma unroll
-                for (int k = 0; k < kRounds; ++k)
-                    if (k < left) vector(k);
+                for (int k = 0; k < kRoundsGrad; ++k)
+                    if (k < left) vector(k, e[k]);
             }
+            ring.release();
         }
     };
+    struct Coef { Pair p[2], q[2], k0[2], k1[2]; };
 
     // z = (x - pivot) p + q as in the forward pass
     auto coefficients = [&](int slice, int64_t image, bool second) {
@@ -670,21 +692,23 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
         Col s0, s1;
 #pragma unroll
         for (int i = 0; i < Col::N; ++i) { s0.e[i] = Col::all(0.f); s1.e[i] = Col::all(0.f); }
-        {
-            Col cs, ch;
-            const int col = w.active ? w.col * VEC : 0;
-            column_load<VEC>(cp + col, cs);
-            column_load<VEC>(cq + col, ch);
-            const Pair np = Col::all(pivots[col]);
-            each(np, [&](const Col &xm, const Col &dc) {
+        const int col = w.active ? w.col * VEC : 0;
+        each(Col::all(pivots[col]),
+             [&](int h) {
+                 Coef c;
+                 quad_load(cp + col + 4 * h, c.p);
+                 quad_load(cq + col + 4 * h, c.q);
+                 return c;
+             },
+             [&](int h, const Coef &c, const Pair (&xm)[2], const Pair (&g)[2], uint4 &) {
 #pragma unroll
-                for (int i = 0; i < Col::N; ++i) {
-                    const Pair dz = act_grad<ACT>(dc.e[i], vfma(xm.e[i], cs.e[i], ch.e[i]), one, minus_one);
-                    s0.e[i] = vadd(s0.e[i], dz);
-                    s1.e[i] = vfma(dz, xm.e[i], s1.e[i]);
-                }
-            });
-        }
+                 for (int i = 0; i < 2; ++i) {
+                     const Pair dz = act_grad<ACT>(g[i], vfma(xm[i], c.p[i], c.q[i]), one);
+                     s0.e[2 * h + i] = vadd(s0.e[2 * h + i], dz);
+                     s1.e[2 * h + i] = vfma(dz, xm[i], s1.e[2 * h + i]);
+                 }
+             },
+             [](const uint4 &) {});
         if (w.active) {
             float *to = buf + w.row * 2 * w.ncols + w.col * VEC;
             column_store<VEC>(to, s0);
@@ -738,25 +762,30 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             if (lane == 0) stat[g] = make_float2(t1 * inv, t2 * inv);
         }
         coefficients(slice, image, true);
-        Col cs, ch, k0, k1;
         const int col = w.active ? w.col * VEC : 0;
-        column_load<VEC>(cp + col, cs);
-        column_load<VEC>(cq + col, ch);
-        column_load<VEC>(c0 + col, k0);
-        column_load<VEC>(c1 + col, k1);
-        const Pair np = Col::all(pivots[col]);
         T *o = dx + image * a.hw * a.channels + slice * w.ncols + mine0;
-        each(np, [&](const Col &xm, Col &dc) {
+        each(Col::all(pivots[col]),
+             [&](int h) {
+                 Coef c;
+                 quad_load(cp + col + 4 * h, c.p);
+                 quad_load(cq + col + 4 * h, c.q);
+                 quad_load(c0 + col + 4 * h, c.k0);
+                 quad_load(c1 + col + 4 * h, c.k1);
+                 return c;
+             },
+             [&](int h, const Coef &c, const Pair (&xm)[2], const Pair (&g)[2], uint4 &r) {
+                 Pair e[2];
 #pragma unroll
-            for (int i = 0; i < Col::N; ++i) {
-                const Pair dz = act_grad<ACT>(dc.e[i], vfma(xm.e[i], cs.e[i], ch.e[i]), one, minus_one);
-                dc.e[i] = vfma(dz, cs.e[i], vfma(xm.e[i], k1.e[i], k0.e[i]));
-            }
-            float f[VEC];
-            dc.get(f);
-            st_stream(o, pack<T>(f));
-            o += step;
-        });
+                 for (int i = 0; i < 2; ++i) {
+                     const Pair dz = act_grad<ACT>(g[i], vfma(xm[i], c.p[i], c.q[i]), one);
+                     e[i] = vfma(dz, c.p[i], vfma(xm[i], c.k1[i], c.k0[i]));
+                 }
+                 half_pack<T>(r, h, e);               // over the half of grad_out that has just been used
+             },
+             [&](const uint4 &r) {
+                 st_stream(o, r);
+                 o += step;
+             });
     };
 
     int summed = -1;                                  // the slice that `total` belongs to
@@ -809,6 +838,12 @@ cl_param_sum_kernel(const float2 *channel_sums, float *grad_gamma, float *grad_b
     }
 }
 
+// (A memset node in front costs 3.5 us of a captured graph's time, a kernel less than 1.)
+__global__ void __launch_bounds__(256) cl_clear_kernel(unsigned int *p, long long n) {
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256)
+        p[i] = 0;
+}
+
 // ---- plan and launch ------------------------------------------------------------------------------
 struct Layout {
     size_t partial, channel_sums, bytes;              // behind the items' counters
@@ -817,7 +852,7 @@ struct Layout {
 Layout layout(const GnClShape &s, const GnClTeamPlan &p, bool backward) {
     const auto up = [](size_t n) { return (n + 15) & ~static_cast<size_t>(15); };
     Layout l;
-    l.partial = up(static_cast<size_t>(s.batch) * p.slices * sizeof(unsigned int));
+    l.partial = up((static_cast<size_t>(s.batch) * p.slices + kSlotWords) * sizeof(unsigned int));
     l.channel_sums = l.partial + up(static_cast<size_t>(s.batch) * s.groups * p.members * sizeof(float2));
     l.bytes = l.channel_sums +
               (backward ? static_cast<size_t>(p.image_teams) * p.members * s.channels * sizeof(float2) : 0);
@@ -834,12 +869,13 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
     a.channels = s.channels;
     a.groups = s.groups;
     a.width = static_cast<int>(s.channels / s.groups);
-    a.chunk_rows = p.rows * kRounds;
+    a.chunk_rows = p.rows * (backward ? kRoundsGrad : kRounds);
     const int64_t chunks = (s.hw + a.chunk_rows - 1) / a.chunk_rows;
     a.share = static_cast<int>(chunks / p.members);
     a.rest = static_cast<int>(chunks % p.members);
     a.eps = s.eps;
     a.arrived = reinterpret_cast<unsigned int *>(base);
+    a.items = s.batch * p.slices;
     a.partial = reinterpret_cast<float2 *>(base + l.partial);
     a.channel_sums = reinterpret_cast<float2 *>(base + l.channel_sums);
     return a;
@@ -848,7 +884,7 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
 size_t shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt) {
     const size_t ncols = static_cast<size_t>(p.cols) * p.vec;
     const size_t vector = !backward ? 16 : ckpt ? 16 + p.vec : 32;
-    return static_cast<size_t>(backward ? kStagesGrad : kStages) * kRounds * kThreads * vector +
+    return static_cast<size_t>(backward ? kStagesGrad * kRoundsGrad : kStages * kRounds) * kThreads * vector +
            (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 10 : 6) * ncols) * sizeof(float);
 }
 
@@ -887,8 +923,11 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t r
 // A cooperative launch: the blocks of a team wait for one another, so either all of them run or none.
 template <typename... Maps>
 cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
-    cudaError_t err = cudaMemsetAsync(a.arrived, 0, static_cast<size_t>(a.batch) * a.p.slices * sizeof(unsigned int), stream);
+    const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
+    cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
+    cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
+    g_launches.fetch_add(1);
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg{};
@@ -970,7 +1009,8 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     }
     p->slices = static_cast<int>(best);
     p->cols = static_cast<int>(grains / best * grain);
-    p->rows = std::min(kThreads / p->cols, 256 / kRounds);                             // a box has at most 256 rows
+    const int rounds = backward ? kRoundsGrad : kRounds;
+    p->rows = std::min(kThreads / p->cols, 256 / rounds);                              // a box has at most 256 rows
     // what an SM holds at once: 228 KB of shared memory, 1 KB of it reserved per block
     const int64_t fit = 228 * 1024 / (static_cast<int64_t>(shared_bytes(*p, backward, ckpt)) + 1024);
     const int64_t blocks = static_cast<int64_t>(sm_count()) * std::min<int64_t>(fit, kBlocksPerSm);
@@ -987,9 +1027,9 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
         if (p->slice_teams > blocks) p->slice_teams = static_cast<int>(blocks);
     }
     int64_t m = std::max<int64_t>(1, blocks / (static_cast<int64_t>(p->slice_teams) * p->image_teams));
-    m = std::min(m, (s.hw + p->rows * kRounds - 1) / (p->rows * kRounds));            // a chunk each at least
+    m = std::min(m, (s.hw + p->rows * rounds - 1) / (p->rows * rounds));            // a chunk each at least
     p->members = static_cast<int>(m);
-    p->lag = m > 1 ? 1 : 0;
+    p->stagger = 0;
     return true;
 }
 
