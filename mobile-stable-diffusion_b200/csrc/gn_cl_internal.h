@@ -15,11 +15,15 @@ cudaError_t gn_cl_split_backward(const GnClShape &s, const GnClBackward &a, void
 struct GnClTeamPlan {
     int vec;               // elements per column: a 16-byte vector
     int cols, rows;        // columns of a slice; rows of threads in a block
+    int rounds;            // rows per thread and chunk
     int slices;            // an image's channels / slice channels
     int slice_teams;       // teams side by side on the slices of an image
     int image_teams;       // teams side by side on images
     int members;           // thread blocks per team
-    int stagger;           // odd teams start behind the even ones' first pass
+    int slice_groups;      // groups of a slice
+    int stagger;           // the odd one of two teams starts behind the even one's first pass
+    int resident;          // one item per team, which fits the ring: read once
+    int cluster;           // a team is a thread-block cluster, one item per team
 };
 // false: no plan for this shape.  pack: the forward pass also writes a checkpoint; ckpt: the
 // backward pass reads one.

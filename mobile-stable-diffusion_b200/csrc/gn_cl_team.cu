@@ -53,10 +53,17 @@ constexpr int kBlock = kThreads + 32;              // and the producer warp
 constexpr int kBlocksPerSm = 2;
 // Rows per thread and chunk, and chunks of the ring.
 constexpr int kRounds = 4, kStages = 5;            // 16 KB chunks
-constexpr int kRoundsGrad = 4, kStagesGrad = 3;    // 16 KB of grad_out and 16, 8 or 4 KB of x or its codes
+// Backward, by the source: 16 KB of grad_out and 8 or 4 KB of codes, or 8 KB of grad_out and 8 KB of x, so that
+// two blocks fit an SM either way (three chunks of 32 KB leave room for one: 35 us instead of 31 at
+// [8, 4096, 320] bf16).
+__host__ __device__ constexpr int rounds_grad(bool ckpt) { return ckpt ? 4 : 2; }
+__host__ __device__ constexpr int stages_grad(bool ckpt) { return ckpt ? 3 : 5; }
 constexpr int kMaxCols = kThreads / 2;             // columns of a slice: a box row of 2 KB
 constexpr int kMergeLoads = 5;                     // a team of up to 160 blocks in one round
-constexpr int64_t kInFlight = 64ll << 20;
+constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward pass
+// Clusters of 8 and 16 start 2 and 7 us later than a cooperative grid, which costs more than their exchange saves.
+constexpr int kMaxCluster = 4;
+constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
 constexpr int kSlotWords = 1024 + kMaxTeamsOfSm;
 
@@ -196,6 +203,10 @@ template <int STAGES> struct Ring {
         if ((threadIdx.x & 31) == 0) mbar_arrive(empty + 8 * stage);
         next();
     }
+    __device__ __forceinline__ void rewind() {           // to the first chunk of a ring that is never released
+        stage = 0;
+        phase = 0;
+    }
     __device__ __forceinline__ void next() {
         if (++stage == STAGES) {
             stage = 0;
@@ -205,6 +216,9 @@ template <int STAGES> struct Ring {
 };
 
 __device__ __forceinline__ void block_sync() { consumer_sync(kThreads); }       // the consumer warps
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ---- exchange ---------------------------------------------------------------------------------------
 // Counts the block in on an item; its sums were written (by any thread) before.
@@ -237,17 +251,47 @@ __device__ __forceinline__ void wait_all(const Args &a, int64_t item) {
 }
 
 // One group's sums of up to 32 * kMergeLoads blocks from `first` on, every load in flight at once.
-__device__ __forceinline__ void load_partials(const Args &a, int64_t group, int first, float2 (&v)[kMergeLoads]) {
-    const float2 *q = a.partial + group * a.p.members + first;
+__device__ __forceinline__ void load_partials(const Args &a, const float2 *sums, int first, float2 (&v)[kMergeLoads]) {
 #pragma unroll
     for (int k = 0; k < kMergeLoads; ++k) {
         v[k] = make_float2(0.f, 0.f);
-        if (first + 32 * k < a.p.members) v[k] = __ldcg(q + 32 * k);
+        if (first + 32 * k < a.p.members) v[k] = __ldcg(sums + first + 32 * k);
     }
+}
+__device__ __forceinline__ void load_parts(const Args &a, const float2 *sums, int lane, float2 (&v)[kMergeLoads]) {
+#pragma unroll
+    for (int k = 0; k < kMergeLoads; ++k) v[k] = make_float2(0.f, 0.f);
+    if (lane < a.p.members) v[0] = sums[lane];
 }
 __device__ __forceinline__ float pixels_or_none(const Args &a, int member) {
     return member < a.p.members ? static_cast<float>(member_pixels(a, member)) : 0.f;
 }
+
+// A team that is a thread-block cluster (one item per team): its blocks put their sums into one another's
+// shared memory, part[group][member], and arrive on one another's barrier.
+struct ClusterExchange {
+    float2 *part;
+    uint32_t bar;
+    __device__ __forceinline__ void init(uint64_t *b, float2 *p, int members) {
+        part = p;
+        bar = smem_addr(b);
+        if (threadIdx.x == 0) {
+            mbar_init(bar, static_cast<uint32_t>(members) * 32u);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    // own[g]: this block's sums, behind a barrier.  Warp m serves member m (and m + 8).
+    __device__ __forceinline__ void send(const Place &w, int members, const float2 *own) const {
+        for (int m = threadIdx.x >> 5; m < members; m += kWarps) {
+            for (int g = threadIdx.x & 31; g < w.slice_groups; g += 32)
+                st_peer_f32x2(map_to_rank(smem_addr(part + g * members + w.member), m), own[g].x, own[g].y);
+            mbar_arrive_peer(map_to_rank(bar, m));
+        }
+    }
+    __device__ __forceinline__ void wait() const {
+        if (!mbar_wait_cluster_bounded(bar, 0u, kWaitCycles)) atomicOr(&g_cl_status, 1u);
+    }
+};
 
 // Odd teams start when half of the blocks of the team before them are through their first pass S.
 __device__ __forceinline__ void stagger(const Args &a, int team) {
@@ -313,7 +357,7 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
 // with P the mean of the thread in row 0: P is close to the block's mean (it can be off by an
 // outlier's share of one thread's pixels, which costs at most log2(rows) bits), so the one
 // subtraction that is left, of N (block mean - P)^2, cancels next to nothing.
-template <typename T, int ACT, bool PACK>
+template <typename T, int ACT, bool PACK, bool CLUSTER>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) {
     constexpr int VEC = VecOf<T>::N;
@@ -328,12 +372,19 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     float *pivots = cq + w.ncols;
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (mean, rstd)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
+    float2 *own = reinterpret_cast<float2 *>(group_of + w.ncols);                        // cluster: [groups], then
+    ClusterExchange cluster;                                                             // [groups][members]
+    __shared__ uint64_t cluster_bar;
+    // a team's only item that fits the ring is read once
+    const bool resident = a.p.resident != 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Passes passes(w);
     Ring<kStages> ring;
     ring.init(bars);
+    if constexpr (CLUSTER) cluster.init(&cluster_bar, own + w.slice_groups, a.p.members);
     for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
     __syncthreads();
+    if constexpr (CLUSTER) cluster_arrive();          // the barriers are set up; waited for before the first store to a peer
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
@@ -341,6 +392,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             const uint64_t again = policy_evict_last(), done = policy_evict_first();
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols * sizeof(T));
             while (passes.next(a, w)) {
+                if (passes.second && resident) break;
                 const int x = static_cast<int>(passes.now.slice * w.ncols * sizeof(T) / 8);
                 const int y = passes.now.image * static_cast<int>(a.hw) + w.first;
                 for (int c = 0; c < w.chunks; ++c, ring.next()) {
@@ -350,6 +402,10 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
                              ring.full + 8 * ring.stage, passes.second ? done : again);
                 }
             }
+        }
+        if constexpr (CLUSTER) {
+            __syncwarp();
+            cluster_wait();                           // every arrival has its wait
         }
         return;
     }
@@ -363,8 +419,9 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     const int round = a.p.rows * a.p.cols;
     const int mine = w.active ? (w.pixels - w.row + a.p.rows - 1) / a.p.rows : 0;
     // one(vector) for each of them
-    auto each = [&](auto one) {
+    auto each = [&](bool again, auto one) {
         int left = mine;
+        if (again) ring.rewind();
         for (int c = 0; c < w.chunks; ++c, left -= kRounds) {
             ring.wait_full();
             const uint4 *p = mine_in + ring.stage * (kChunkBytes / 16);
@@ -374,7 +431,8 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             } else {
                 for (int k = 0; k < left; ++k) one(p[k * round]);
             }
-            ring.release();
+            if (resident) ring.next();
+            else ring.release();
         }
     };
 
@@ -391,7 +449,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             nk.set(f);
         }
         int64_t at = image * a.hw * a.channels + slice * w.ncols + mine0;
-        each([&](const uint4 &v) {
+        each(false, [&](const uint4 &v) {
             float f[VEC];
             unpack<T>(v, f);
             if constexpr (PACK) {
@@ -454,15 +512,25 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
                 u += fmaxf(fmaf(-buf[c], e, buf[w.ncols + c]), 0.f) + pixels * d * d;
             }
             u = seg.sum(u);
-            if (seg.lane == 0 && g < w.slice_groups) __stcg(a.partial + (group0 + g) * a.p.members + w.member, make_float2(mu, u));
+            if (seg.lane == 0 && g < w.slice_groups) {
+                if constexpr (CLUSTER) own[g] = make_float2(mu, u);
+                else __stcg(a.partial + (group0 + g) * a.p.members + w.member, make_float2(mu, u));
+            }
         }
-        arrive(a, image * a.p.slices + slice);
+        if constexpr (CLUSTER) {
+            block_sync();
+            cluster_wait();
+            cluster.send(w, a.p.members, own);
+        } else {
+            arrive(a, image * a.p.slices + slice);
+        }
     };
 
     // z = (x - pivot) p + q, the pivot being the mean of the column's first channel: where the mean is far
     // from zero compared with the spread, x - pivot loses nothing, and one register serves the vector.
     auto apply = [&](int slice, int64_t image) {
-        wait_all(a, image * a.p.slices + slice);
+        if constexpr (CLUSTER) cluster.wait();
+        else wait_all(a, image * a.p.slices + slice);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float hw = static_cast<float>(a.hw), width = static_cast<float>(a.width);
         for (int g = warp; g < w.slice_groups; g += kWarps) {
@@ -470,7 +538,8 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             float mu = 0.f, u = 0.f, n = 0.f;
             for (int first = 0; first < a.p.members; first += 32 * kMergeLoads) {
                 float2 v[kMergeLoads];
-                load_partials(a, group0 + g, first + lane, v);
+                if constexpr (CLUSTER) load_parts(a, cluster.part + g * a.p.members, lane, v);
+                else load_partials(a, a.partial + (group0 + g) * a.p.members, first + lane, v);
                 float t = 0.f, px = 0.f;
 #pragma unroll
                 for (int k = 0; k < kMergeLoads; ++k) {
@@ -515,7 +584,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
         const int col = w.active ? w.col * VEC : 0;
         const Pair np = Col::all(pivots[col]);
         T *o = y + image * a.hw * a.channels + slice * w.ncols + mine0;
-        each([&](const uint4 &v) {
+        each(resident, [&](const uint4 &v) {
             uint4 r;
 #pragma unroll
             for (int h = 0; h < VEC / 4; ++h) {
@@ -539,10 +608,11 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
 }
 
 // ---- backward -------------------------------------------------------------------------------------
-template <typename T, int ACT, bool CKPT>
+template <typename T, int ACT, bool CKPT, bool CLUSTER>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy) {
     constexpr int VEC = VecOf<T>::N;
+    constexpr int kRoundsGrad = rounds_grad(CKPT), kStagesGrad = stages_grad(CKPT);
     constexpr int kBytes = kRoundsGrad * kThreads * 16;                  // grad_out's part of a chunk
     constexpr int kBytesX = CKPT ? kRoundsGrad * kThreads * VEC : kBytes;
     constexpr int kChunkBytes = kBytes + kBytesX;
@@ -560,12 +630,19 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     float *pivots = c1 + w.ncols;
     float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (s1, s2)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
+    float2 *own = reinterpret_cast<float2 *>(group_of + w.ncols);                        // cluster: [groups], then
+    ClusterExchange cluster;                                                             // [groups][members]
+    __shared__ uint64_t cluster_bar;
+    // a team's only item that fits the ring is read once
+    const bool resident = a.p.resident != 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Passes passes(w);
     Ring<kStagesGrad> ring;
     ring.init(bars);
+    if constexpr (CLUSTER) cluster.init(&cluster_bar, own + w.slice_groups, a.p.members);
     for (int c = threadIdx.x; c < w.ncols; c += kBlock) group_of[c] = c / a.width;
     __syncthreads();
+    if constexpr (CLUSTER) cluster_arrive();          // the barriers are set up; waited for before the first store to a peer
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
@@ -574,6 +651,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             constexpr int kSizeX = CKPT ? 1 : sizeof(T);
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols) * (sizeof(T) + kSizeX);
             while (passes.next(a, w)) {
+                if (passes.second && resident) break;
                 const int x = static_cast<int>(passes.now.slice * w.ncols * sizeof(T) / 8);
                 const int xx = passes.now.slice * w.ncols * kSizeX / 8;
                 const int y = passes.now.image * static_cast<int>(a.hw) + w.first;
@@ -586,6 +664,10 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
                     box_load(to + kBytes, &map_x, xx, y + c * a.chunk_rows, bar, policy);
                 }
             }
+        }
+        if constexpr (CLUSTER) {
+            __syncwarp();
+            cluster_wait();                           // every arrival has its wait
         }
         return;
     }
@@ -621,8 +703,9 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     // use(h, coefficients, x - pivot, grad_out, vector) for both halves of each of this thread's vectors, then
     // done(vector).  The coefficients are read from shared memory where they are used: held in
     // registers they would take a third of the warps away.
-    auto each = [&](Pair np, auto coefficient, auto use, auto done) {
+    auto each = [&](bool again, Pair np, auto coefficient, auto use, auto done) {
         int left = mine;
+        if (again) ring.rewind();
         for (int c = 0; c < w.chunks; ++c, left -= kRoundsGrad) {
             ring.wait_full();
             const unsigned char *p = shared + ring.stage * kChunkBytes;
@@ -660,7 +743,8 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
                 for (int k = 0; k < kRoundsGrad; ++k)
                     if (k < left) vector(k, e[k]);
             }
-            ring.release();
+            if (resident) ring.next();
+            else ring.release();
         }
     };
     struct Coef { Pair p[2], q[2], k0[2], k1[2]; };
@@ -693,7 +777,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
 #pragma unroll
         for (int i = 0; i < Col::N; ++i) { s0.e[i] = Col::all(0.f); s1.e[i] = Col::all(0.f); }
         const int col = w.active ? w.col * VEC : 0;
-        each(Col::all(pivots[col]),
+        each(false, Col::all(pivots[col]),
              [&](int h) {
                  Coef c;
                  quad_load(cp + col + 4 * h, c.p);
@@ -736,21 +820,32 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             }
             t1 = seg.sum(t1);
             t2 = seg.sum(t2);
-            if (seg.lane == 0 && g < w.slice_groups) __stcg(a.partial + (group0 + g) * a.p.members + w.member, make_float2(t1, t2));
+            if (seg.lane == 0 && g < w.slice_groups) {
+                if constexpr (CLUSTER) own[g] = make_float2(t1, t2);
+                else __stcg(a.partial + (group0 + g) * a.p.members + w.member, make_float2(t1, t2));
+            }
         }
-        arrive(a, image * a.p.slices + slice);
+        if constexpr (CLUSTER) {
+            block_sync();
+            cluster_wait();
+            cluster.send(w, a.p.members, own);
+        } else {
+            arrive(a, image * a.p.slices + slice);
+        }
     };
 
     auto apply = [&](int slice, int64_t image) {
         first_scales(slice, image);
-        wait_all(a, image * a.p.slices + slice);
+        if constexpr (CLUSTER) cluster.wait();
+        else wait_all(a, image * a.p.slices + slice);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float inv = 1.0f / (static_cast<float>(a.hw) * static_cast<float>(a.width));
         for (int g = warp; g < w.slice_groups; g += kWarps) {
             float t1 = 0.f, t2 = 0.f;
             for (int first = 0; first < a.p.members; first += 32 * kMergeLoads) {
                 float2 v[kMergeLoads];
-                load_partials(a, group0 + g, first + lane, v);
+                if constexpr (CLUSTER) load_parts(a, cluster.part + g * a.p.members, lane, v);
+                else load_partials(a, a.partial + (group0 + g) * a.p.members, first + lane, v);
 #pragma unroll
                 for (int k = 0; k < kMergeLoads; ++k) {
                     t1 += v[k].x;
@@ -764,7 +859,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
         coefficients(slice, image, true);
         const int col = w.active ? w.col * VEC : 0;
         T *o = dx + image * a.hw * a.channels + slice * w.ncols + mine0;
-        each(Col::all(pivots[col]),
+        each(resident, Col::all(pivots[col]),
              [&](int h) {
                  Coef c;
                  quad_load(cp + col + 4 * h, c.p);
@@ -852,8 +947,9 @@ struct Layout {
 Layout layout(const GnClShape &s, const GnClTeamPlan &p, bool backward) {
     const auto up = [](size_t n) { return (n + 15) & ~static_cast<size_t>(15); };
     Layout l;
-    l.partial = up((static_cast<size_t>(s.batch) * p.slices + kSlotWords) * sizeof(unsigned int));
-    l.channel_sums = l.partial + up(static_cast<size_t>(s.batch) * s.groups * p.members * sizeof(float2));
+    l.partial = p.cluster ? 0 : up((static_cast<size_t>(s.batch) * p.slices + kSlotWords) * sizeof(unsigned int));
+    l.channel_sums =
+        l.partial + (p.cluster ? 0 : up(static_cast<size_t>(s.batch) * s.groups * p.members * sizeof(float2)));
     l.bytes = l.channel_sums +
               (backward ? static_cast<size_t>(p.image_teams) * p.members * s.channels * sizeof(float2) : 0);
     return l;
@@ -869,7 +965,7 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
     a.channels = s.channels;
     a.groups = s.groups;
     a.width = static_cast<int>(s.channels / s.groups);
-    a.chunk_rows = p.rows * (backward ? kRoundsGrad : kRounds);
+    a.chunk_rows = p.rows * p.rounds;
     const int64_t chunks = (s.hw + a.chunk_rows - 1) / a.chunk_rows;
     a.share = static_cast<int>(chunks / p.members);
     a.rest = static_cast<int>(chunks % p.members);
@@ -884,8 +980,9 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
 size_t shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt) {
     const size_t ncols = static_cast<size_t>(p.cols) * p.vec;
     const size_t vector = !backward ? 16 : ckpt ? 16 + p.vec : 32;
-    return static_cast<size_t>(backward ? kStagesGrad * kRoundsGrad : kStages * kRounds) * kThreads * vector +
-           (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 10 : 6) * ncols) * sizeof(float);
+    return static_cast<size_t>(backward ? stages_grad(ckpt) * rounds_grad(ckpt) : kStages * kRounds) * kThreads * vector +
+           (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 10 : 6) * ncols) * sizeof(float) +
+           (p.cluster ? static_cast<size_t>(p.slice_groups) * (1 + p.members) * sizeof(float2) : 0);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -920,14 +1017,18 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t r
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// A cooperative launch: the blocks of a team wait for one another, so either all of them run or none.
+// A team is a cluster, or else the launch is cooperative: the blocks of a team wait for one another, so
+// either all of them run or none.
 template <typename... Maps>
 cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
-    const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
-    cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
-    cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return err;
-    g_launches.fetch_add(1);
+    cudaError_t err;
+    if (!a.p.cluster) {
+        const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
+        cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
+        err = cudaGetLastError();
+        if (err != cudaSuccess) return err;
+        g_launches.fetch_add(1);
+    }
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg{};
@@ -936,28 +1037,35 @@ cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cu
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
+    if (a.p.cluster) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(a.p.members);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+    } else {
+        attr[0].id = cudaLaunchAttributeCooperative;
+        attr[0].val.cooperative = 1;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = a.p.members > 1 ? 1 : 0;
+    cfg.numAttrs = 1;
     err = cudaLaunchKernelEx(&cfg, kernel, a, maps...);
     if (err == cudaSuccess) g_launches.fetch_add(1);
     return err;
 }
 
-template <typename T> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
     CUtensorMap x;
     const cudaError_t err = make_map(&x, a.f.in, s.batch * s.hw, s.channels * sizeof(T), a.p.cols * 16, a.chunk_rows);
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, false, false);
     if (s.act == kActSilu)
-        return a.f.codes ? launch(cl_team_forward_kernel<T, kActSilu, true>, a, smem, stream, x)
-                         : launch(cl_team_forward_kernel<T, kActSilu, false>, a, smem, stream, x);
-    return a.f.codes ? launch(cl_team_forward_kernel<T, kActNone, true>, a, smem, stream, x)
-                     : launch(cl_team_forward_kernel<T, kActNone, false>, a, smem, stream, x);
+        return a.f.codes ? launch(cl_team_forward_kernel<T, kActSilu, true, CLUSTER>, a, smem, stream, x)
+                         : launch(cl_team_forward_kernel<T, kActSilu, false, CLUSTER>, a, smem, stream, x);
+    return a.f.codes ? launch(cl_team_forward_kernel<T, kActNone, true, CLUSTER>, a, smem, stream, x)
+                     : launch(cl_team_forward_kernel<T, kActNone, false, CLUSTER>, a, smem, stream, x);
 }
 
-template <typename T> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
     const int64_t rows = s.batch * s.hw, row_bytes = s.channels * sizeof(T);
     CUtensorMap x, dy;
     cudaError_t err = make_map(&dy, a.b.grad_out, rows, row_bytes, a.p.cols * 16, a.chunk_rows);
@@ -967,10 +1075,10 @@ template <typename T> cudaError_t backward_type(const GnClShape &s, Args &a, cud
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, true, a.b.codes != nullptr);
     if (s.act == kActSilu)
-        return a.b.codes ? launch(cl_team_backward_kernel<T, kActSilu, true>, a, smem, stream, x, dy)
-                         : launch(cl_team_backward_kernel<T, kActSilu, false>, a, smem, stream, x, dy);
-    return a.b.codes ? launch(cl_team_backward_kernel<T, kActNone, true>, a, smem, stream, x, dy)
-                     : launch(cl_team_backward_kernel<T, kActNone, false>, a, smem, stream, x, dy);
+        return a.b.codes ? launch(cl_team_backward_kernel<T, kActSilu, true, CLUSTER>, a, smem, stream, x, dy)
+                         : launch(cl_team_backward_kernel<T, kActSilu, false, CLUSTER>, a, smem, stream, x, dy);
+    return a.b.codes ? launch(cl_team_backward_kernel<T, kActNone, true, CLUSTER>, a, smem, stream, x, dy)
+                     : launch(cl_team_backward_kernel<T, kActNone, false, CLUSTER>, a, smem, stream, x, dy);
 }
 
 }  // namespace
@@ -990,46 +1098,65 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     const int64_t grains = s.channels / grain;
     grain /= p->vec;
     if (grain > kMaxCols) return false;
+    const int64_t grain_bytes = grain * p->vec * esize;
+    const int64_t want = (128 + grain_bytes - 1) / grain_bytes;                       // grains per slice
+    p->rounds = backward ? rounds_grad(ckpt) : kRounds;
+    const int stages = backward ? stages_grad(ckpt) : kStages;
+    const auto allowed = [&](int64_t d) { return grains % d == 0 && grains / d * grain <= kMaxCols; };
+    const auto set_slices = [&](int64_t d) {
+        p->slices = static_cast<int>(d);
+        p->cols = static_cast<int>(grains / d * grain);
+        p->rows = std::min(kThreads / p->cols, 256 / p->rounds);                       // a box has at most 256 rows
+        p->slice_groups = static_cast<int>(p->cols * p->vec / width);
+        return (s.hw + p->rows * p->rounds - 1) / (p->rows * p->rounds);               // chunks of an item
+    };
+    p->stagger = p->resident = p->cluster = 0;
+    const int64_t sms = sm_count();
+
+    // Small tensors: one item per cluster, read once, no workspace.  Of the slices and cluster sizes that do with
+    // one wave of blocks the one with the most blocks, and of those the widest rows.
+    int64_t best = 0, best_slices = 0, best_members = 0;
+    for (int64_t d = 1; d <= grains; ++d) {
+        if (!allowed(d) || (d > 1 && grains / d * grain_bytes < 64)) continue;
+        const int64_t n = set_slices(d);
+        for (int64_t m = 1; m <= kMaxCluster; m *= 2) {
+            const int64_t blocks = s.batch * d * m;
+            if (blocks > sms * kBlocksPerSm || m > n || (n + m - 1) / m > stages || blocks <= best ||
+                static_cast<int64_t>(p->slice_groups) * (m + 1) * 8 > kClusterPartBytes)
+                continue;
+            best = blocks, best_slices = d, best_members = m;
+        }
+    }
+    if (best > 0) {
+        set_slices(best_slices);
+        p->cluster = p->resident = 1;
+        p->slice_teams = static_cast<int>(best_slices);
+        p->image_teams = static_cast<int>(s.batch);
+        p->members = static_cast<int>(best_members);
+        return true;
+    }
+
+    // slices: as many as leave rows of 128 bytes, but few enough that all images that fit L2 have their teams
     const int64_t per_element = backward ? (ckpt ? 1 : esize) + esize : esize;
     const int64_t image = s.hw * s.channels * per_element;
-    // slices: as many as leave rows of 128 bytes, more only where an image is too large for L2 twice
-    const int64_t grain_bytes = grain * p->vec * esize;
-    const int64_t want = (128 + grain_bytes - 1) / grain_bytes;                         // grains per slice
-    const int64_t least = (2 * image + kInFlight - 1) / kInFlight;                      // slices
-    int64_t best = 0;
-    for (int64_t d = 1; d <= grains; ++d) {                                            // slices
-        if (grains % d != 0 || grains / d * grain > kMaxCols) continue;
-        if (best == 0 || grains / d >= want || (d >= least && best < least && grains / d * grain * p->vec * esize >= 64)) best = d;
-    }
-    if (best == 0) return false;
-    // large images: only as many slices as the footprint asks for
-    if (least > 1) {
-        for (int64_t d = 1; d <= best; ++d)
-            if (grains % d == 0 && grains / d * grain <= kMaxCols && d >= least) { best = d; break; }
-    }
-    p->slices = static_cast<int>(best);
-    p->cols = static_cast<int>(grains / best * grain);
-    const int rounds = backward ? kRoundsGrad : kRounds;
-    p->rows = std::min(kThreads / p->cols, 256 / rounds);                              // a box has at most 256 rows
+    const int64_t in_flight = backward ? 2 * kInFlight : kInFlight;
+    const int64_t images = std::min(s.batch, std::max<int64_t>(1, in_flight / image));
+    int64_t slices = 0;
+    for (int64_t d = 1; d <= grains; ++d)
+        if (allowed(d) && (slices == 0 || (grains / d >= want && d * images <= sms * kBlocksPerSm))) slices = d;
+    if (slices == 0) return false;
+    const int64_t chunks = set_slices(slices);
     // what an SM holds at once: 228 KB of shared memory, 1 KB of it reserved per block
     const int64_t fit = 228 * 1024 / (static_cast<int64_t>(shared_bytes(*p, backward, ckpt)) + 1024);
-    const int64_t blocks = static_cast<int64_t>(sm_count()) * std::min<int64_t>(fit, kBlocksPerSm);
-    if (least > 1) {
-        p->slice_teams = 1;
-        p->image_teams = 1;
-    } else {
-        p->slice_teams = static_cast<int>(best);
-        int64_t n = s.batch * image <= kInFlight ? s.batch : std::max<int64_t>(1, kInFlight / (2 * image));
-        n = std::min(n, std::max<int64_t>(1, blocks / best));
-        n = std::min(n, s.batch);
-        n = (s.batch + (s.batch + n - 1) / n - 1) / ((s.batch + n - 1) / n);           // even rounds
-        p->image_teams = static_cast<int>(n);
-        if (p->slice_teams > blocks) p->slice_teams = static_cast<int>(blocks);
-    }
-    int64_t m = std::max<int64_t>(1, blocks / (static_cast<int64_t>(p->slice_teams) * p->image_teams));
-    m = std::min(m, (s.hw + p->rows * rounds - 1) / (p->rows * rounds));            // a chunk each at least
-    p->members = static_cast<int>(m);
-    p->stagger = 0;
+    const int64_t blocks = sms * std::min<int64_t>(fit, kBlocksPerSm);
+    p->slice_teams = static_cast<int>(std::min(slices, std::max<int64_t>(1, in_flight * slices / image)));
+    while (slices % p->slice_teams != 0) --p->slice_teams;
+    int64_t n = std::min(images, std::max<int64_t>(1, blocks / p->slice_teams));
+    n = (s.batch + (s.batch + n - 1) / n - 1) / ((s.batch + n - 1) / n);               // even rounds
+    p->image_teams = static_cast<int>(n);
+    p->members = static_cast<int>(std::min(std::max<int64_t>(1, blocks / (p->slice_teams * n)), chunks));
+    p->resident = slices == p->slice_teams && s.batch == n && (chunks + p->members - 1) / p->members <= stages;
+    p->stagger = !p->resident && p->slice_teams * n == kMaxTeamsOfSm && p->members == sms && fit >= kBlocksPerSm;
     return true;
 }
 
@@ -1041,9 +1168,9 @@ cudaError_t gn_cl_team_forward(const GnClShape &s, const GnClTeamPlan &p, const 
     Args a = make_args(s, p, false, ws);
     a.f = f;
     switch (s.dtype) {
-        case kF16: return forward_type<__half>(s, a, stream);
-        case kBF16: return forward_type<__nv_bfloat16>(s, a, stream);
-        default: return forward_type<float>(s, a, stream);
+        case kF16: return p.cluster ? forward_type<__half, true>(s, a, stream) : forward_type<__half, false>(s, a, stream);
+        case kBF16: return p.cluster ? forward_type<__nv_bfloat16, true>(s, a, stream) : forward_type<__nv_bfloat16, false>(s, a, stream);
+        default: return p.cluster ? forward_type<float, true>(s, a, stream) : forward_type<float, false>(s, a, stream);
     }
 }
 
@@ -1053,9 +1180,9 @@ cudaError_t gn_cl_team_backward(const GnClShape &s, const GnClTeamPlan &p, const
     a.b = b;
     cudaError_t err;
     switch (s.dtype) {
-        case kF16: err = backward_type<__half>(s, a, stream); break;
-        case kBF16: err = backward_type<__nv_bfloat16>(s, a, stream); break;
-        default: err = backward_type<float>(s, a, stream); break;
+        case kF16: err = p.cluster ? backward_type<__half, true>(s, a, stream) : backward_type<__half, false>(s, a, stream); break;
+        case kBF16: err = p.cluster ? backward_type<__nv_bfloat16, true>(s, a, stream) : backward_type<__nv_bfloat16, false>(s, a, stream); break;
+        default: err = p.cluster ? backward_type<float, true>(s, a, stream) : backward_type<float, false>(s, a, stream); break;
     }
     if (err != cudaSuccess || (!b.grad_gamma && !b.grad_beta)) return err;
     cl_param_sum_kernel<<<static_cast<unsigned>((s.channels + 31) / 32), kThreads, 0, stream>>>(
