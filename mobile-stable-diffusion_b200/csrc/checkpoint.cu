@@ -19,6 +19,11 @@ namespace sdfl {
 namespace {
 
 constexpr int kCkThreads = 256;
+constexpr int kVecs = 4;             // vectors per thread and round: pack, expand
+constexpr int kGateVecs = 2;         // of each half: gate
+constexpr int kElems = 4;            // elements per lane: element kernels of pack and expand
+constexpr int kElemBlocks = 32 * kElems / kCkptBlock;      // blocks of a warp at a time
+constexpr int kElemRounds = 2;       // of those, loads first
 
 inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -39,25 +44,36 @@ pack_vec_kernel(const uint4 *__restrict__ src, typename CodeVec<VecOf<T>::N>::ty
                 uint8_t *__restrict__ scales, long long nslots, uint32_t slots_row, FastDiv slots_div, uint32_t vecs_row) {
     constexpr int VEC = VecOf<T>::N;
     constexpr int LANES = kCkptBlock / VEC;
-    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads * kVecs;
     // whole warps go round together: the shuffles need every lane
-    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads + (threadIdx.x & ~31); base < nslots;
+    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads * kVecs + (threadIdx.x & ~31); base < nslots;
          base += stride) {
-        const long long i = base + (threadIdx.x & 31);
-        long long at = i;
-        bool live = i < nslots;
-        if (RAGGED) {
-            const uint32_t row = slots_div.div(static_cast<uint32_t>(i));
-            const uint32_t col = static_cast<uint32_t>(i) - row * slots_row;
-            live = live && col < vecs_row;
-            at = static_cast<long long>(row) * vecs_row + col;
+        long long at[kVecs];
+        bool live[kVecs];
+        uint4 v[kVecs];
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            const long long i = base + k * kCkThreads + (threadIdx.x & 31);
+            at[k] = i;
+            live[k] = i < nslots;
+            if (RAGGED) {
+                const uint32_t row = slots_div.div(static_cast<uint32_t>(i));
+                const uint32_t col = static_cast<uint32_t>(i) - row * slots_row;
+                live[k] = live[k] && col < vecs_row;
+                at[k] = static_cast<long long>(row) * vecs_row + col;
+            }
+            v[k] = live[k] ? ld_stream(src + at[k]) : make_uint4(0, 0, 0, 0);
         }
-        float f[VEC];
-        unpack<T>(live ? ld_stream(src + at) : make_uint4(0, 0, 0, 0), f);
-        const CkptScale s = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
-        if (live) {
-            codes[at] = ckpt_codes(f, s);
-            if ((threadIdx.x & (LANES - 1)) == 0) scales[i / LANES] = static_cast<uint8_t>(s.e);
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            float f[VEC];
+            unpack<T>(v[k], f);
+            const CkptScale s = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
+            if (live[k]) {
+                codes[at[k]] = ckpt_codes(f, s);
+                if ((threadIdx.x & (LANES - 1)) == 0)
+                    scales[(base + k * kCkThreads + (threadIdx.x & 31)) / LANES] = static_cast<uint8_t>(s.e);
+            }
         }
     }
 }
@@ -65,19 +81,42 @@ pack_vec_kernel(const uint4 *__restrict__ src, typename CodeVec<VecOf<T>::N>::ty
 template <typename T>
 __global__ void __launch_bounds__(kCkThreads)
 pack_element_kernel(const T *__restrict__ src, int8_t *__restrict__ codes, uint8_t *__restrict__ scales,
-                    long long nblocks, long long dim, long long blocks_row) {
-    const int lane = threadIdx.x & 31;
-    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32);
-    for (long long b = static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); b < nblocks;
-         b += stride) {
-        const long long row = b / blocks_row, col = (b - row * blocks_row) * kCkptBlock + lane;
-        const bool live = col < dim;
-        const float x = live ? to_float<T>(src[row * dim + col]) : 0.f;
-        const CkptScale s = ckpt_scale(__reduce_max_sync(0xffffffffu, abs_bits(x)));
-        if (live) codes[row * dim + col] = static_cast<int8_t>(ckpt_code(x, s.inv) & s.keep);
-        if (lane == 0) scales[b] = static_cast<uint8_t>(s.e);
+                    long long nblocks, long long dim, long long blocks_row, FastDiv row_div, bool narrow) {
+    constexpr uint32_t LANES = kCkptBlock / kElems;
+    const uint32_t lane = threadIdx.x & 31;
+    const long long step = static_cast<long long>(kElemBlocks) * kElemRounds;
+    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32) * step;
+    for (long long first = (static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
+         first < nblocks; first += stride) {
+        long long at[kElemRounds];
+        int left[kElemRounds];                        // of this lane's elements, those inside the row
+        float x[kElemRounds][kElems];
+#pragma unroll
+        for (int r = 0; r < kElemRounds; ++r) {
+            const long long b = first + r * kElemBlocks + lane / LANES;
+            const long long row = narrow ? row_div.div(static_cast<uint32_t>(b)) : b / blocks_row;
+            const long long col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            at[r] = row * dim + col;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<long long>(kElems))) : 0;
+#pragma unroll
+            for (int k = 0; k < kElems; ++k) x[r][k] = k < left[r] ? to_float<T>(src[at[r] + k]) : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < kElemRounds; ++r) {
+            const long long b = first + r * kElemBlocks + lane / LANES;
+            const CkptScale s = ckpt_scale(block_lanes_max<kElems>(max_abs_bits<kElems>(x[r])));
+#pragma unroll
+            for (int k = 0; k < kElems; ++k)
+                if (k < left[r]) codes[at[r] + k] = static_cast<int8_t>(ckpt_code(x[r][k], s.inv) & s.keep);
+            if (lane % LANES == 0 && b < nblocks) scales[b] = static_cast<uint8_t>(s.e);
+        }
     }
 }
+
+// Division of a block number by the blocks of a row: multiply-high while the numbers fit 31 bits (with room for
+// the last round's overhang), a 64-bit division beyond.
+inline bool narrow_blocks(int64_t nblocks) { return nblocks + kElemBlocks * kElemRounds < (1ll << 31); }
+inline unsigned element_grid(int64_t nblocks) { return ck_grid((nblocks + kElemRounds * kElemBlocks - 1) / (kElemRounds * kElemBlocks) * 32); }
 
 template <typename T>
 cudaError_t pack_dispatch(const void *src, int8_t *codes, uint8_t *scales, int64_t rows, int64_t dim,
@@ -88,16 +127,18 @@ cudaError_t pack_dispatch(const void *src, int8_t *codes, uint8_t *scales, int64
     const int64_t slots_row = blocks_row * (kCkptBlock / VEC), nslots = rows * slots_row;
     const bool vec = dim % VEC == 0 && aligned(src, 16) && aligned(codes, VEC);
     if (vec && dim % kCkptBlock == 0) {
-        pack_vec_kernel<T, false><<<ck_grid(nslots), kCkThreads, 0, stream>>>(
+        pack_vec_kernel<T, false><<<ck_grid((nslots + kVecs - 1) / kVecs), kCkThreads, 0, stream>>>(
             static_cast<const uint4 *>(src), reinterpret_cast<CV *>(codes), scales, nslots, 1, FastDiv::make(1), 1);
-    } else if (vec && nslots < (1ll << 31)) {
-        pack_vec_kernel<T, true><<<ck_grid(nslots), kCkThreads, 0, stream>>>(
+    } else if (vec && nslots < (1ll << 31) - kVecs * kCkThreads) {
+        pack_vec_kernel<T, true><<<ck_grid((nslots + kVecs - 1) / kVecs), kCkThreads, 0, stream>>>(
             static_cast<const uint4 *>(src), reinterpret_cast<CV *>(codes), scales, nslots,
             static_cast<uint32_t>(slots_row), FastDiv::make(static_cast<uint32_t>(slots_row)),
             static_cast<uint32_t>(dim / VEC));
     } else {
-        pack_element_kernel<T><<<ck_grid(nblocks * 32), kCkThreads, 0, stream>>>(static_cast<const T *>(src), codes, scales,
-                                                                                nblocks, dim, blocks_row);
+        const bool narrow = narrow_blocks(nblocks);
+        pack_element_kernel<T><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+            static_cast<const T *>(src), codes, scales, nblocks, dim, blocks_row,
+            FastDiv::make(narrow ? static_cast<uint32_t>(blocks_row) : 1), narrow);
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
@@ -111,30 +152,64 @@ unpack_vec_kernel(const typename CodeVec<VecOf<T>::N>::type *__restrict__ codes,
                   uint4 *__restrict__ dst, long long nvec, uint32_t vecs_row, FastDiv vecs_div, uint32_t blocks_row) {
     constexpr int VEC = VecOf<T>::N;
     constexpr int LANES = kCkptBlock / VEC;
-    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
-    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < nvec; i += stride) {
-        long long block = i / LANES;
-        if (RAGGED) {
-            const uint32_t row = vecs_div.div(static_cast<uint32_t>(i));
-            const uint32_t col = static_cast<uint32_t>(i) - row * vecs_row;
-            block = static_cast<long long>(row) * blocks_row + col / LANES;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads * kVecs;
+    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads * kVecs + threadIdx.x; base < nvec; base += stride) {
+        typename CodeVec<VEC>::type c[kVecs];
+        uint8_t e[kVecs];
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            const long long i = base + k * kCkThreads;
+            if (i >= nvec) continue;
+            long long block = i / LANES;
+            if (RAGGED) {
+                const uint32_t row = vecs_div.div(static_cast<uint32_t>(i));
+                const uint32_t col = static_cast<uint32_t>(i) - row * vecs_row;
+                block = static_cast<long long>(row) * blocks_row + col / LANES;
+            }
+            c[k] = __ldcs(codes + i);
+            e[k] = __ldg(scales + block);
         }
-        float f[VEC];
-        ckpt_values(__ldcs(codes + i), ckpt_step(__ldg(scales + block)), f);
-        st_stream(dst + i, pack<T>(f));
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            const long long i = base + k * kCkThreads;
+            if (i >= nvec) continue;
+            float f[VEC];
+            ckpt_values(c[k], ckpt_step(e[k]), f);
+            st_stream(dst + i, pack<T>(f));
+        }
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kCkThreads)
 unpack_element_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales, T *__restrict__ dst,
-                      long long nblocks, long long dim, long long blocks_row) {
-    const int lane = threadIdx.x & 31;
-    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32);
-    for (long long b = static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); b < nblocks;
-         b += stride) {
-        const long long row = b / blocks_row, col = (b - row * blocks_row) * kCkptBlock + lane;
-        if (col < dim) dst[row * dim + col] = from_float<T>(ckpt_value(codes[row * dim + col], scales[b]));
+                      long long nblocks, long long dim, long long blocks_row, FastDiv row_div, bool narrow) {
+    constexpr uint32_t LANES = kCkptBlock / kElems;
+    const uint32_t lane = threadIdx.x & 31;
+    const long long step = static_cast<long long>(kElemBlocks) * kElemRounds;
+    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32) * step;
+    for (long long first = (static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
+         first < nblocks; first += stride) {
+        long long at[kElemRounds];
+        int left[kElemRounds];
+        int8_t c[kElemRounds][kElems];
+        uint8_t e[kElemRounds];
+#pragma unroll
+        for (int r = 0; r < kElemRounds; ++r) {
+            const long long b = first + r * kElemBlocks + lane / LANES;
+            const long long row = narrow ? row_div.div(static_cast<uint32_t>(b)) : b / blocks_row;
+            const long long col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            at[r] = row * dim + col;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<long long>(kElems))) : 0;
+            e[r] = b < nblocks ? scales[b] : 0;
+#pragma unroll
+            for (int k = 0; k < kElems; ++k) c[r][k] = k < left[r] ? codes[at[r] + k] : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < kElemRounds; ++r)
+#pragma unroll
+            for (int k = 0; k < kElems; ++k)
+                if (k < left[r]) dst[at[r] + k] = from_float<T>(ckpt_value(c[r][k], e[r]));
     }
 }
 
@@ -147,15 +222,17 @@ cudaError_t unpack_dispatch(const int8_t *codes, const uint8_t *scales, void *ds
     const int64_t vecs_row = dim / VEC, nvec = rows * vecs_row;
     const bool vec = dim % VEC == 0 && aligned(dst, 16) && aligned(codes, VEC);
     if (vec && dim % kCkptBlock == 0) {
-        unpack_vec_kernel<T, false><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+        unpack_vec_kernel<T, false><<<ck_grid((nvec + kVecs - 1) / kVecs), kCkThreads, 0, stream>>>(
             reinterpret_cast<const CV *>(codes), scales, static_cast<uint4 *>(dst), nvec, 1, FastDiv::make(1), 1);
     } else if (vec && nvec < (1ll << 31)) {
-        unpack_vec_kernel<T, true><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
+        unpack_vec_kernel<T, true><<<ck_grid((nvec + kVecs - 1) / kVecs), kCkThreads, 0, stream>>>(
             reinterpret_cast<const CV *>(codes), scales, static_cast<uint4 *>(dst), nvec, static_cast<uint32_t>(vecs_row),
             FastDiv::make(static_cast<uint32_t>(vecs_row)), static_cast<uint32_t>(blocks_row));
     } else {
-        unpack_element_kernel<T><<<ck_grid(nblocks * 32), kCkThreads, 0, stream>>>(codes, scales, static_cast<T *>(dst),
-                                                                                  nblocks, dim, blocks_row);
+        const bool narrow = narrow_blocks(nblocks);
+        unpack_element_kernel<T><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+            codes, scales, static_cast<T *>(dst), nblocks, dim, blocks_row,
+            FastDiv::make(narrow ? static_cast<uint32_t>(blocks_row) : 1), narrow);
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
@@ -163,9 +240,9 @@ cudaError_t unpack_dispatch(const int8_t *codes, const uint8_t *scales, void *ds
 }
 
 // ---- GEGLU gate with a checkpoint of its input [rows, 2 D] -----------------------------------------
-// D a multiple of 32, so that no block holds elements of both halves.  The gate itself is the
-// arithmetic of gelu_multiply: the same bits come out.
-template <typename T>
+// PACK: D a multiple of 32, so that no block holds elements of both halves; otherwise the gate alone, and
+// pack_dispatch does the rest.  The gate itself is the arithmetic of gelu_multiply: the same bits come out.
+template <typename T, bool PACK>
 __global__ void __launch_bounds__(kCkThreads)
 geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
                   typename CodeVec<VecOf<T>::N>::type *__restrict__ codes, uint8_t *__restrict__ scales,
@@ -173,42 +250,58 @@ geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
     constexpr int VEC = VecOf<T>::N;
     constexpr int LANES = kCkptBlock / VEC;
     constexpr bool HALF = sizeof(T) == 2;
-    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads;
-    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads + (threadIdx.x & ~31); base < nvec;
+    const long long stride = static_cast<long long>(gridDim.x) * kCkThreads * kGateVecs;
+    for (long long base = static_cast<long long>(blockIdx.x) * kCkThreads * kGateVecs + (threadIdx.x & ~31); base < nvec;
          base += stride) {
-        const long long i = base + (threadIdx.x & 31);
-        const bool live = i < nvec;
-        const uint32_t r = dvec_div.div(static_cast<uint32_t>(live ? i : 0));
-        const uint32_t j = static_cast<uint32_t>(live ? i : 0) - r * dvec;
-        const long long at = static_cast<long long>(r) * 2 * dvec + j;
-        float a[VEC], g[VEC];
-        unpack<T>(live ? ld_stream(ab + at) : make_uint4(0, 0, 0, 0), a);
-        unpack<T>(live ? ld_stream(ab + at + dvec) : make_uint4(0, 0, 0, 0), g);
-        const CkptScale sa = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(a)));
-        const CkptScale sg = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(g)));
-        if (live) {
-            codes[at] = ckpt_codes(a, sa);
-            codes[at + dvec] = ckpt_codes(g, sg);
-            if ((threadIdx.x & (LANES - 1)) == 0) {
-                scales[at / LANES] = static_cast<uint8_t>(sa.e);
-                scales[(at + dvec) / LANES] = static_cast<uint8_t>(sg.e);
-            }
+        long long at[kGateVecs];
+        uint4 va[kGateVecs], vg[kGateVecs];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) a[k] = a[k] * gelu_erf<HALF>(g[k]);
-            st_stream(dst + i, pack<T>(a));
+        for (int k = 0; k < kGateVecs; ++k) {
+            const long long i = base + k * kCkThreads + (threadIdx.x & 31);
+            const uint32_t n = static_cast<uint32_t>(i < nvec ? i : 0);
+            const uint32_t r = dvec_div.div(n);
+            at[k] = static_cast<long long>(r) * 2 * dvec + (n - r * dvec);
+            va[k] = vg[k] = make_uint4(0, 0, 0, 0);
+            if (i < nvec) {
+                va[k] = ld_stream(ab + at[k]);
+                vg[k] = ld_stream(ab + at[k] + dvec);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kGateVecs; ++k) {
+            const long long i = base + k * kCkThreads + (threadIdx.x & 31);
+            float a[VEC], g[VEC];
+            unpack<T>(va[k], a);
+            unpack<T>(vg[k], g);
+            if constexpr (PACK) {
+                const CkptScale sa = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(a)));
+                const CkptScale sg = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(g)));
+                if (i < nvec) {
+                    codes[at[k]] = ckpt_codes(a, sa);
+                    codes[at[k] + dvec] = ckpt_codes(g, sg);
+                    if ((threadIdx.x & (LANES - 1)) == 0) {
+                        scales[at[k] / LANES] = static_cast<uint8_t>(sa.e);
+                        scales[(at[k] + dvec) / LANES] = static_cast<uint8_t>(sg.e);
+                    }
+                }
+            }
+            if (i < nvec) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) a[j] = a[j] * gelu_erf<HALF>(g[j]);
+                st_stream(dst + i, pack<T>(a));
+            }
         }
     }
 }
 
-// The gate alone, element by element: with pack_dispatch the two-launch form for shapes that the
-// fused kernel does not take.
+// The gate alone, element by element, for rows that are not whole vectors.
 template <typename T>
 __global__ void __launch_bounds__(kCkThreads)
-geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, long long rows, long long d) {
+geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, long long rows, long long d, FastDiv row_div, bool narrow) {
     constexpr bool HALF = sizeof(T) == 2;
     const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
     for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const long long r = i / d, j = i - r * d;
+        const long long r = narrow ? row_div.div(static_cast<uint32_t>(i)) : i / d, j = i - r * d;
         dst[i] = from_float<T>(to_float<T>(ab[r * 2 * d + j]) * gelu_erf<HALF>(to_float<T>(ab[r * 2 * d + d + j])));
     }
 }
@@ -219,17 +312,26 @@ cudaError_t geglu_pack_dispatch(const void *ab, void *dst, int8_t *codes, uint8_
     constexpr int VEC = VecOf<T>::N;
     using CV = typename CodeVec<VEC>::type;
     const int64_t nvec = rows * (d / VEC);
-    if (d % kCkptBlock == 0 && aligned(ab, 16) && aligned(dst, 16) && aligned(codes, VEC) && nvec < (1ll << 31)) {
+    if (d % VEC == 0 && aligned(ab, 16) && aligned(dst, 16) && nvec < (1ll << 31)) {
         const uint32_t dvec = static_cast<uint32_t>(d / VEC);
-        geglu_pack_kernel<T><<<ck_grid(nvec), kCkThreads, 0, stream>>>(
-            static_cast<const uint4 *>(ab), static_cast<uint4 *>(dst), reinterpret_cast<CV *>(codes), scales, nvec,
-            FastDiv::make(dvec), dvec);
+        const unsigned grid = ck_grid((nvec + kGateVecs - 1) / kGateVecs);
+        const bool pack = d % kCkptBlock == 0 && aligned(codes, VEC);
+        if (pack)
+            geglu_pack_kernel<T, true><<<grid, kCkThreads, 0, stream>>>(
+                static_cast<const uint4 *>(ab), static_cast<uint4 *>(dst), reinterpret_cast<CV *>(codes), scales, nvec,
+                FastDiv::make(dvec), dvec);
+        else
+            geglu_pack_kernel<T, false><<<grid, kCkThreads, 0, stream>>>(static_cast<const uint4 *>(ab),
+                                                                        static_cast<uint4 *>(dst), nullptr, nullptr, nvec,
+                                                                        FastDiv::make(dvec), dvec);
         cudaError_t err = cudaGetLastError();
-        if (err == cudaSuccess) g_launches.fetch_add(1);
-        return err;
+        if (err != cudaSuccess) return err;
+        g_launches.fetch_add(1);
+        return pack ? cudaSuccess : pack_dispatch<T>(ab, codes, scales, rows, 2 * d, stream);
     }
-    geglu_element_kernel<T><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(static_cast<const T *>(ab), static_cast<T *>(dst),
-                                                                          rows, d);
+    const bool narrow = rows * d < (1ll << 31);
+    geglu_element_kernel<T><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+        static_cast<const T *>(ab), static_cast<T *>(dst), rows, d, FastDiv::make(narrow ? static_cast<uint32_t>(d) : 1), narrow);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     g_launches.fetch_add(1);
@@ -239,7 +341,8 @@ cudaError_t geglu_pack_dispatch(const void *ab, void *dst, int8_t *codes, uint8_
 // ---- backward of the gate -----------------------------------------------------------------------
 // y = a gelu(g), gelu(g) = g Phi(g):  da = dy g Phi(g),  dg = dy a (Phi(g) + g phi(g)).
 // Phi for half storage from the same rational approximation as the forward's erf, taken as the tail
-// probability first (no cancellation for negative g); phi shares its exponential.  fp32 storage uses erfcf.
+// probability first (no cancellation for negative g); phi shares its exponential.  fp32 storage
+// uses erff, as its forward does (erfcf is 15 % slower over the whole kernel and gains nothing next to |dy g| 2^-24).
 template <bool HALF> __device__ __forceinline__ void gelu_grad(float g, float *value, float *slope) {
     float cdf, pdf;
     if (HALF) {
@@ -254,8 +357,8 @@ template <bool HALF> __device__ __forceinline__ void gelu_grad(float g, float *v
         cdf = g < 0.f ? tail : 1.0f - tail;
         pdf = e * 0.39894228040143267794f;
     } else {
-        cdf = 0.5f * erfcf(g * -0.70710678118654752440f);
-        pdf = expf(-0.5f * g * g) * 0.39894228040143267794f;
+        cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752440f));
+        pdf = ex2_approx(-0.72134752044448170368f * g * g) * 0.39894228040143267794f;
     }
     *value = g * cdf;
     *slope = fmaf(g, pdf, cdf);
@@ -301,11 +404,12 @@ geglu_backward_vec_kernel(const uint4 *ab, const typename CodeVec<VecOf<T>::N>::
 template <typename T, bool CKPT>
 __global__ void __launch_bounds__(kCkThreads)
 geglu_backward_element_kernel(const T *ab, const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                              const T *dy, T *dab, long long rows, long long d, long long blocks_row) {
+                              const T *dy, T *dab, long long rows, long long d, long long blocks_row, FastDiv row_div,
+                              bool narrow) {
     constexpr bool HALF = sizeof(T) == 2;
     const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
     for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const long long r = i / d, j = i - r * d, at = r * 2 * d + j;
+        const long long r = narrow ? row_div.div(static_cast<uint32_t>(i)) : i / d, j = i - r * d, at = r * 2 * d + j;
         float a, g;
         if (CKPT) {
             a = ckpt_value(codes[at], scales[r * blocks_row + j / kCkptBlock]);
@@ -335,9 +439,10 @@ cudaError_t geglu_backward_dispatch(const void *ab, const int8_t *codes, const u
             static_cast<const uint4 *>(ab), reinterpret_cast<const CV *>(codes), scales, static_cast<const uint4 *>(dy),
             static_cast<uint4 *>(dab), nvec, FastDiv::make(dvec), dvec, static_cast<uint32_t>(blocks_row));
     } else {
+        const bool narrow = rows * d < (1ll << 31);
         geglu_backward_element_kernel<T, CKPT><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
             static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab), rows, d,
-            blocks_row);
+            blocks_row, FastDiv::make(narrow ? static_cast<uint32_t>(d) : 1), narrow);
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
