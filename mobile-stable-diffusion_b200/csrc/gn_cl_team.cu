@@ -63,6 +63,7 @@ constexpr int kMergeLoads = 5;                     // a team of up to 160 blocks
 constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward pass
 // Clusters of 8 and 16 start 2 and 7 us later than a cooperative grid, which costs more than their exchange saves.
 constexpr int kMaxCluster = 4;
+constexpr size_t kMaxShared = 200 * 1024;
 constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
 constexpr int kSlotWords = 1024 + kMaxTeamsOfSm;
@@ -179,7 +180,9 @@ template <int STAGES> struct Ring {
     uint32_t full, empty;        // shared addresses of STAGES mbarriers each
     int stage;
     uint32_t phase;
+    long long patience;          // of a wait; short once one has run out, so that a broken launch ends soon
     __device__ __forceinline__ void init(uint64_t *bars) {
+        patience = kWaitCycles;
         full = smem_addr(bars);
         empty = full + 8 * STAGES;
         stage = 0;
@@ -193,7 +196,10 @@ template <int STAGES> struct Ring {
         }
     }
     __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
-        if (!mbar_wait_bounded(bar + 8 * stage, parity, kWaitCycles)) atomicOr(&g_cl_status, 1u);
+        if (!mbar_wait_bounded(bar + 8 * stage, parity, patience)) {
+            atomicOr(&g_cl_status, 1u);
+            patience = kWaitCyclesAfterTimeout;
+        }
     }
     __device__ __forceinline__ void wait_full() { wait(full, phase); }
     __device__ __forceinline__ void wait_empty() { wait(empty, phase ^ 1u); }
@@ -230,14 +236,16 @@ __device__ __forceinline__ void arrive(const Args &a, int64_t item) {
     }
 }
 
-__device__ __forceinline__ void wait_count(const Args &a, int64_t item, unsigned int count, unsigned int sleep) {
+__device__ __forceinline__ void wait_count(const Args &a, int64_t item, unsigned int count, unsigned int sleep,
+                                           long long &patience) {
     const long long t0 = clock64();
     for (;;) {
         unsigned int v;
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(a.arrived + item) : "memory");
         if (v >= count) break;
-        if (clock64() - t0 > kWaitCycles) {
+        if (clock64() - t0 > patience) {
             atomicOr(&g_cl_status, 1u);
+            patience = kWaitCyclesAfterTimeout;
             break;
         }
         if (sleep) __nanosleep(sleep);
@@ -245,8 +253,8 @@ __device__ __forceinline__ void wait_count(const Args &a, int64_t item, unsigned
 }
 
 // Waits until all of the team's blocks have counted themselves in.
-__device__ __forceinline__ void wait_all(const Args &a, int64_t item) {
-    if (threadIdx.x == 0) wait_count(a, item, static_cast<unsigned>(a.p.members), 0);
+__device__ __forceinline__ void wait_all(const Args &a, int64_t item, long long &patience) {
+    if (threadIdx.x == 0) wait_count(a, item, static_cast<unsigned>(a.p.members), 0, patience);
     block_sync();
 }
 
@@ -294,11 +302,11 @@ struct ClusterExchange {
 };
 
 // Odd teams start when half of the blocks of the team before them are through their first pass S.
-__device__ __forceinline__ void stagger(const Args &a, int team) {
+__device__ __forceinline__ void stagger(const Args &a, int team, long long &patience) {
     if (!a.p.stagger || !(team & 1)) return;
     const int before = team - 1;
     wait_count(a, static_cast<int64_t>(before / a.p.slice_teams) * a.p.slices + before % a.p.slice_teams,
-               static_cast<unsigned>((a.p.members + 1) / 2), 200);
+               static_cast<unsigned>((a.p.members + 1) / 2), 200, patience);
 }
 
 // Groups of a slice are dealt to segments of L lanes, L the largest power of two up to the group's width.
@@ -388,7 +396,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
-            stagger(a, w.team);
+            stagger(a, w.team, ring.patience);
             const uint64_t again = policy_evict_last(), done = policy_evict_first();
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols * sizeof(T));
             while (passes.next(a, w)) {
@@ -530,7 +538,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     // from zero compared with the spread, x - pivot loses nothing, and one register serves the vector.
     auto apply = [&](int slice, int64_t image) {
         if constexpr (CLUSTER) cluster.wait();
-        else wait_all(a, image * a.p.slices + slice);
+        else wait_all(a, image * a.p.slices + slice, ring.patience);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float hw = static_cast<float>(a.hw), width = static_cast<float>(a.width);
         for (int g = warp; g < w.slice_groups; g += kWarps) {
@@ -646,7 +654,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
-            stagger(a, w.team);
+            stagger(a, w.team, ring.patience);
             const uint64_t again = policy_evict_last(), done = policy_evict_first();
             constexpr int kSizeX = CKPT ? 1 : sizeof(T);
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols) * (sizeof(T) + kSizeX);
@@ -837,7 +845,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     auto apply = [&](int slice, int64_t image) {
         first_scales(slice, image);
         if constexpr (CLUSTER) cluster.wait();
-        else wait_all(a, image * a.p.slices + slice);
+        else wait_all(a, image * a.p.slices + slice, ring.patience);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         const float inv = 1.0f / (static_cast<float>(a.hw) * static_cast<float>(a.width));
         for (int g = warp; g < w.slice_groups; g += kWarps) {
@@ -1019,8 +1027,8 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t r
 
 // A team is a cluster, or else the launch is cooperative: the blocks of a team wait for one another, so
 // either all of them run or none.
-template <typename... Maps>
-cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
+template <auto kernel, typename... Maps>
+cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
     cudaError_t err;
     if (!a.p.cluster) {
         const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
@@ -1029,8 +1037,17 @@ cudaError_t launch(void (*kernel)(Args, Maps...), const Args &a, size_t smem, cu
         if (err != cudaSuccess) return err;
         g_launches.fetch_add(1);
     }
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // once per kernel and device, to what any of its plans may ask for
+    static std::atomic<bool> prepared[kMaxDevices];
+    int dev = 0;
+    err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    if (dev >= kMaxDevices || !prepared[dev].load(std::memory_order_relaxed)) {
+        err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+        if (err != cudaSuccess) return err;
+        if (dev < kMaxDevices) prepared[dev].store(true, std::memory_order_relaxed);
+    }
+    if (smem > kMaxShared) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.p.slice_teams * a.p.image_teams * a.p.members));
     cfg.blockDim = dim3(kBlock);
@@ -1059,10 +1076,10 @@ template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s,
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, false, false);
     if (s.act == kActSilu)
-        return a.f.codes ? launch(cl_team_forward_kernel<T, kActSilu, true, CLUSTER>, a, smem, stream, x)
-                         : launch(cl_team_forward_kernel<T, kActSilu, false, CLUSTER>, a, smem, stream, x);
-    return a.f.codes ? launch(cl_team_forward_kernel<T, kActNone, true, CLUSTER>, a, smem, stream, x)
-                     : launch(cl_team_forward_kernel<T, kActNone, false, CLUSTER>, a, smem, stream, x);
+        return a.f.codes ? launch<cl_team_forward_kernel<T, kActSilu, true, CLUSTER>>(a, smem, stream, x)
+                         : launch<cl_team_forward_kernel<T, kActSilu, false, CLUSTER>>(a, smem, stream, x);
+    return a.f.codes ? launch<cl_team_forward_kernel<T, kActNone, true, CLUSTER>>(a, smem, stream, x)
+                     : launch<cl_team_forward_kernel<T, kActNone, false, CLUSTER>>(a, smem, stream, x);
 }
 
 template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
@@ -1075,10 +1092,10 @@ template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, true, a.b.codes != nullptr);
     if (s.act == kActSilu)
-        return a.b.codes ? launch(cl_team_backward_kernel<T, kActSilu, true, CLUSTER>, a, smem, stream, x, dy)
-                         : launch(cl_team_backward_kernel<T, kActSilu, false, CLUSTER>, a, smem, stream, x, dy);
-    return a.b.codes ? launch(cl_team_backward_kernel<T, kActNone, true, CLUSTER>, a, smem, stream, x, dy)
-                     : launch(cl_team_backward_kernel<T, kActNone, false, CLUSTER>, a, smem, stream, x, dy);
+        return a.b.codes ? launch<cl_team_backward_kernel<T, kActSilu, true, CLUSTER>>(a, smem, stream, x, dy)
+                         : launch<cl_team_backward_kernel<T, kActSilu, false, CLUSTER>>(a, smem, stream, x, dy);
+    return a.b.codes ? launch<cl_team_backward_kernel<T, kActNone, true, CLUSTER>>(a, smem, stream, x, dy)
+                     : launch<cl_team_backward_kernel<T, kActNone, false, CLUSTER>>(a, smem, stream, x, dy);
 }
 
 }  // namespace
