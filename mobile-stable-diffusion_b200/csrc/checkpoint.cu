@@ -66,10 +66,10 @@ pack_vec_kernel(const uint4 *__restrict__ src, typename CodeVec<VecOf<T>::N>::ty
         }
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) {
-            float f[VEC];
-            unpack<T>(v[k], f);
-            const CkptScale s = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
+            const CkptScale s = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<T>(v[k])));
             if (live[k]) {
+                float f[VEC];
+                unpack<T>(v[k], f);
                 codes[at[k]] = ckpt_codes(f, s);
                 if ((threadIdx.x & (LANES - 1)) == 0)
                     scales[(base + k * kCkThreads + (threadIdx.x & 31)) / LANES] = static_cast<uint8_t>(s.e);
@@ -274,8 +274,8 @@ geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
             unpack<T>(va[k], a);
             unpack<T>(vg[k], g);
             if constexpr (PACK) {
-                const CkptScale sa = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(a)));
-                const CkptScale sg = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(g)));
+                const CkptScale sa = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<T>(va[k])));
+                const CkptScale sg = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<T>(vg[k])));
                 if (i < nvec) {
                     codes[at[k]] = ckpt_codes(a, sa);
                     codes[at[k] + dvec] = ckpt_codes(g, sg);

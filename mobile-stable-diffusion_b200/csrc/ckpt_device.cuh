@@ -18,6 +18,8 @@
 
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace sdfl {
 
 namespace {
@@ -37,10 +39,25 @@ template <int N> __device__ __forceinline__ uint32_t max_abs_bits(const float (&
     return m;
 }
 
+// The same of a vector as it is stored; 16-bit types two at a time, since without their signs they
+// order like integers as well.
+template <typename T> __device__ __forceinline__ uint32_t max_abs_bits(const uint4 &v) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    } else {
+        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        const uint16_t top = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+        if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(top)));
+        else return static_cast<uint32_t>(top) << 16;
+    }
+}
+
 struct CkptScale {
     uint32_t e;        // the scale byte
     float inv;         // 1 / step
     uint32_t keep;     // all ones, or 0 for a block with a non-finite element
+    bool edge;         // the largest element is 127.5 steps or more: codes may need the clamp
 };
 
 __device__ __forceinline__ CkptScale ckpt_scale(uint32_t amax_bits) {
@@ -50,6 +67,7 @@ __device__ __forceinline__ CkptScale ckpt_scale(uint32_t amax_bits) {
     s.e = bad ? kCkptNonFinite : max(ex, 13u) - 6u;          // >= 7: step >= 2^-120
     s.inv = bad ? 0.f : __uint_as_float((254u - s.e) << 23);
     s.keep = bad ? 0u : 0xffffffffu;
+    s.edge = (amax_bits & 0x7fffffu) >= 0x7f0000u;
     return s;
 }
 
@@ -60,9 +78,16 @@ __device__ __forceinline__ uint32_t ckpt_code(float x, float inv) {
     return __float_as_uint(fminf(fmaxf(fmaf(x, inv, kMagic), kMagic - 127.0f), kMagic + 127.0f));
 }
 
+// Without the clamp: right wherever no element of the block reaches 127.5 steps, which is all but one block in
+// 180 of evenly spread mantissas.  The clamp's two operations per element run on the pipe that
+// bounds the packing kernels, so whole vectors go one way or the other.
+__device__ __forceinline__ uint32_t ckpt_code_inside(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.0f)); }
+
+template <bool CLAMP>
 __device__ __forceinline__ uint32_t ckpt_code4(float a, float b, float c, float d, const CkptScale &s) {
-    const uint32_t lo = __byte_perm(ckpt_code(a, s.inv), ckpt_code(b, s.inv), 0x0040);
-    const uint32_t hi = __byte_perm(ckpt_code(c, s.inv), ckpt_code(d, s.inv), 0x0040);
+    const auto code = [&](float x) { return CLAMP ? ckpt_code(x, s.inv) : ckpt_code_inside(x, s.inv); };
+    const uint32_t lo = __byte_perm(code(a), code(b), 0x0040);
+    const uint32_t hi = __byte_perm(code(c), code(d), 0x0040);
     return __byte_perm(lo, hi, 0x5410) & s.keep;
 }
 
@@ -92,10 +117,12 @@ __device__ __forceinline__ void ckpt_values(const uint32_t &w, float step, float
     ckpt_values4(w, step, f);
 }
 __device__ __forceinline__ uint2 ckpt_codes(const float (&f)[8], const CkptScale &s) {
-    return make_uint2(ckpt_code4(f[0], f[1], f[2], f[3], s), ckpt_code4(f[4], f[5], f[6], f[7], s));
+    if (s.edge)
+        return make_uint2(ckpt_code4<true>(f[0], f[1], f[2], f[3], s), ckpt_code4<true>(f[4], f[5], f[6], f[7], s));
+    return make_uint2(ckpt_code4<false>(f[0], f[1], f[2], f[3], s), ckpt_code4<false>(f[4], f[5], f[6], f[7], s));
 }
 __device__ __forceinline__ uint32_t ckpt_codes(const float (&f)[4], const CkptScale &s) {
-    return ckpt_code4(f[0], f[1], f[2], f[3], s);
+    return s.edge ? ckpt_code4<true>(f[0], f[1], f[2], f[3], s) : ckpt_code4<false>(f[0], f[1], f[2], f[3], s);
 }
 
 // Maximum over the 32 / N neighbouring lanes that hold one block (N elements per lane, the first

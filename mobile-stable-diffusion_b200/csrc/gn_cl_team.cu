@@ -461,7 +461,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             float f[VEC];
             unpack<T>(v, f);
             if constexpr (PACK) {
-                const CkptScale sc = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<VEC>(f)));
+                const CkptScale sc = ckpt_scale(block_lanes_max<VEC>(max_abs_bits<T>(v)));
                 *reinterpret_cast<typename CodeVec<VEC>::type *>(a.f.codes + at) = ckpt_codes(f, sc);
                 if ((w.col & (kCkptBlock / VEC - 1)) == 0) a.f.scales[at / kCkptBlock] = static_cast<uint8_t>(sc.e);
                 at += step;

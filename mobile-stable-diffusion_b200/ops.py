@@ -569,8 +569,11 @@ class Checkpoint8:
 
 def _empty_checkpoint(x: torch.Tensor) -> Checkpoint8:
     shape = x.shape
-    return Checkpoint8(torch.empty_like(x, dtype=torch.int8),
-                       x.new_empty(shape[:-1] + (-(-shape[-1] // 32),), dtype=torch.uint8), x.dtype)
+    kept = object.__new__(Checkpoint8)                # the constructor's checks hold by construction
+    kept.codes = torch.empty_like(x, dtype=torch.int8)
+    kept.scales = x.new_empty(shape[:-1] + (-(-shape[-1] // 32),), dtype=torch.uint8)
+    kept.dtype = x.dtype
+    return kept
 
 
 def _source_on(index: int, source) -> tuple:
