@@ -1,5 +1,6 @@
 """B200 (sm_100a) fused layer kernels of a Stable Diffusion pipeline: GroupNorm(+SiLU),
-LayerNorm, GEGLU / gelu / quick_gelu / SiLU, token+position embedding, timestep embedding.
+LayerNorm, GEGLU / gelu / quick_gelu / SiLU, token+position embedding, timestep embedding; for training,
+channels-last GroupNorm(+SiLU) with its gradient, 8-bit activation checkpoints and the GEGLU gradient.
 
 The product is ``lib/libsdfl.so`` (C ABI: ``include/sdfl.h``); this package is the thin host
 side: a ctypes binding (``_capi``), tensor-level wrappers (``ops``), the reference-shaped
