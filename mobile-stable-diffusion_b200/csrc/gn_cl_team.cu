@@ -61,8 +61,10 @@ __host__ __device__ constexpr int stages_grad(bool ckpt) { return ckpt ? 3 : 5; 
 constexpr int kMaxCols = kThreads / 2;             // columns of a slice: a box row of 2 KB
 constexpr int kMergeLoads = 5;                     // a team of up to 160 blocks in one round
 constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward pass
-// Clusters of 8 and 16 start 2 and 7 us later than a cooperative grid, which costs more than their exchange saves.
-constexpr int kMaxCluster = 4;
+// Clusters of up to 4 start as fast as single blocks.  Clusters of 8 start 2 us later, so that [2, 4096, 320]
+// fp16 takes 12.1 us in a captured graph where a cooperative grid takes 11.0, but the call is one launch
+// instead of two: 13 us against 16 when calls are made one by one.  Clusters of 16 start 7 us later.
+constexpr int kMaxCluster = 8;
 constexpr size_t kMaxShared = 200 * 1024;
 constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
@@ -1133,17 +1135,18 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     // Small tensors: one item per cluster, read once, no workspace.  Of the slices and cluster sizes that do with
     // one wave of blocks the one with the most blocks, and of those the widest rows.
     int64_t best = 0, best_slices = 0, best_members = 0;
-    for (int64_t d = 1; d <= grains; ++d) {
-        if (!allowed(d) || (d > 1 && grains / d * grain_bytes < 64)) continue;
-        const int64_t n = set_slices(d);
-        for (int64_t m = 1; m <= kMaxCluster; m *= 2) {
-            const int64_t blocks = s.batch * d * m;
-            if (blocks > sms * kBlocksPerSm || m > n || (n + m - 1) / m > stages || blocks <= best ||
-                static_cast<int64_t>(p->slice_groups) * (m + 1) * 8 > kClusterPartBytes)
-                continue;
-            best = blocks, best_slices = d, best_members = m;
+    for (int64_t limit = kMaxCluster / 2; limit <= kMaxCluster && best == 0; limit *= 2)
+        for (int64_t d = 1; d <= grains; ++d) {
+            if (!allowed(d) || (d > 1 && grains / d * grain_bytes < 64)) continue;
+            const int64_t n = set_slices(d);
+            for (int64_t m = 1; m <= limit; m *= 2) {
+                const int64_t blocks = s.batch * d * m;
+                if (blocks > sms * kBlocksPerSm || m > n || (n + m - 1) / m > stages || blocks <= best ||
+                    static_cast<int64_t>(p->slice_groups) * (m + 1) * 8 > kClusterPartBytes)
+                    continue;
+                best = blocks, best_slices = d, best_members = m;
+            }
         }
-    }
     if (best > 0) {
         set_slices(best_slices);
         p->cluster = p->resident = 1;
