@@ -1,18 +1,31 @@
 // Channels-last GroupNorm (+SiLU) and its gradient in one persistent launch (plus a small one that adds
 // up the weight gradients).  Formulas and layout: gn_cl_device.cuh.
 //
-// What bounds it: HBM.  The forward pass cannot do without one read and one write of the tensor, the
-// backward pass without reads of x (or its checkpoint) and grad_out and one write; but both have to
-// see a whole group before the first result, so every element is read twice.  The kernel keeps
-// the second read inside L2.
+// What it cannot do without is one read and one write of the tensor (forward), or reads of x (or its
+// checkpoint) and grad_out and one write (backward); but a group's first result needs its last element,
+// so every element is read twice, the second time from shared memory or from L2.  What bounds the
+// forward pass is the sum of the HBM reads of pass S, the L2 reads, arithmetic and stores of pass A and the
+// exchange between them ([4, 262144, 128] fp16 with SiLU: S alone 52 us, 5.1 TB/s; A's loads and the
+// exchange 42; A's arithmetic and stores, which overlap, 40).  The backward pass is bound by issue slots:
+// about 15 instructions per element and pass at 0.6 per cycle.
+// Measured (B200, back to back in a captured graph; share of the measured copy bandwidth by the bytes above):
+//   forward   [4, 262144, 128] fp16 SiLU 128 us (65 %), [8, 4096, 512] fp16 26 us (41 %), [3, 2961, 640] fp32 17 us
+//             (42 %), [2, 64, 1280] fp16 7.8 us; with a checkpoint [4, 16384, 512] fp16 48 us (55 %)
+//   backward  [2, 262144, 64] fp32 110 us (57 %), [8, 4096, 320] bf16 32 us (31 %), [4, 1024, 640] bf16 15 us;
+//             from a checkpoint [4, 65536, 256] bf16 121 us (43 %), [4, 16384, 512] fp16 67 us (39 %)
 //
 // Split.  An item is a slice of an image's channels (whole groups and whole vectors, a 128-byte row or
-// more where the sizes allow it) over all its pixels.  A team of M thread blocks goes through its items
-// together, each block on its own range of pixels: pass S reads and sums, the blocks' sums are exchanged,
-// pass A reads again and writes.  The bytes of all teams' open items stay below kInFlight, so that the
-// second read comes from L2 whatever the tensor's size.  An SM holds blocks of two teams, the odd ones
-// started behind the even ones' first pass S, so that one team's reading, which waits for HBM, and its
-// exchange run beside the other's writing, which computes.
+// more where the sizes allow it) over all its pixels.  A team of M thread blocks works on one item at a
+// time, each block on its own range of pixels: pass S reads and sums, the blocks' sums are exchanged,
+// pass A reads again and writes.
+//   - Small tensors: one item per team, its share of it in a block's shared memory and read once; a team is
+//     a thread-block cluster and the exchange goes through distributed shared memory: one launch, no
+//     workspace.
+//   - Otherwise teams of resident blocks.  If all items fit the rings at once they are read once; if not, the
+//     images that are open at a time hold at most kInFlight bytes, so that the second read comes from L2
+//     whatever the tensor's size.  Where that leaves two teams of one block per SM, the second starts
+//     behind the first one's pass S, so that one team's reading, which waits for HBM, runs beside the
+//     other's writing, which computes (134 -> 128 us).
 // (Alternating the chunks of S of one item with those of A of another in the same block was tried and is
 // 15 % slower: three items per team are open then, so they are smaller, and what a block spends per
 // item -- about 5 us for adding up and exchanging -- is paid more often.)
@@ -24,7 +37,7 @@
 // pass are already under way.  The copies cost the consumers no issue slots, and those are what the
 // gradient runs short of first (per-thread cp.async into the same ring: 12 more instructions per vector).
 //
-// Exchange.  A block writes its sums per group to the workspace and counts itself in (the counters are
+// Exchange outside clusters.  A block writes its sums per group to the workspace and counts itself in (the counters are
 // zeroed by a small kernel in front); before pass A one thread of a block polls the count, then
 // the block merges all of the team's sums itself, in block order (the same bits on every run).  Every
 // block of the grid is resident (cooperative launch), and every wait is bounded: on time-out the
@@ -232,7 +245,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Counts the block in on an item; its sums were written (by any thread) before.
 __device__ __forceinline__ void arrive(const Args &a, int64_t item) {
     block_sync();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && a.p.members > 1) {        // a team of one has read its own sums behind the barrier
         __threadfence();
         atomicAdd(a.arrived + item, 1u);
     }
@@ -256,7 +269,7 @@ __device__ __forceinline__ void wait_count(const Args &a, int64_t item, unsigned
 
 // Waits until all of the team's blocks have counted themselves in.
 __device__ __forceinline__ void wait_all(const Args &a, int64_t item, long long &patience) {
-    if (threadIdx.x == 0) wait_count(a, item, static_cast<unsigned>(a.p.members), 0, patience);
+    if (threadIdx.x == 0 && a.p.members > 1) wait_count(a, item, static_cast<unsigned>(a.p.members), 0, patience);
     block_sync();
 }
 
@@ -1032,7 +1045,8 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t r
 template <auto kernel, typename... Maps>
 cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
     cudaError_t err;
-    if (!a.p.cluster) {
+    const bool counted = !a.p.cluster && a.p.members > 1;
+    if (counted) {
         const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
         cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
         err = cudaGetLastError();
@@ -1056,7 +1070,7 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    if (a.p.cluster) {
+    if (!counted) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = static_cast<unsigned>(a.p.members);
         attr[0].val.clusterDim.y = 1;
