@@ -7,7 +7,7 @@
 // forward pass is the sum of the HBM reads of pass S, the L2 reads, arithmetic and stores of pass A and the
 // exchange between them ([4, 262144, 128] fp16 with SiLU: S alone 52 us, 5.1 TB/s; A's loads and the
 // exchange 42; A's arithmetic and stores, which overlap, 40).  The backward pass is bound by issue slots:
-// about 15 instructions per element and pass at 0.6 per cycle.
+// about 18 instructions per element and pass at 0.56 per cycle and scheduler.
 // Measured (B200, back to back in a captured graph; share of the measured copy bandwidth by the bytes above):
 //   forward   [4, 262144, 128] fp16 SiLU 128 us (65 %), [8, 4096, 512] fp16 26 us (41 %), [3, 2961, 640] fp32 17 us
 //             (42 %), [2, 64, 1280] fp16 7.8 us; with a checkpoint [4, 16384, 512] fp16 48 us (55 %)
