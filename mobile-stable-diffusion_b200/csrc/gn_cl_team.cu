@@ -580,7 +580,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
                 }
                 e = warp_sum(e);
                 const float d = m - mu, f = px / (n + px);
-                u += e + d * d * n * width * f;
+                u += e + d * (d * (n * width * f));     // n is 0 in the first round, and d may be large
                 mu = fmaf(d, f, mu);
                 n += px;
             }

@@ -716,7 +716,7 @@ def groupnorm_channels_last_backward(grad_out: torch.Tensor, source, mean: torch
         out = torch.empty_like(grad_out)
     elif out.shape != grad_out.shape or out.dtype != grad_out.dtype:
         raise ValueError("out must match grad_out in shape and dtype")
-    grad_gamma, grad_beta = torch.empty_like(gamma), torch.empty_like(gamma)
+    grad_gamma, grad_beta = torch.empty_like(gamma), torch.empty_like(beta)
     nbytes = _gn_cl_workspace_bytes(index, B, Cc, hw, num_groups, 1, code)
     pw = None
     if nbytes:

@@ -123,6 +123,23 @@ def test_large_offset_and_outliers(sdfl, P, C, G):
         assert_within(y, want, half_step(want, "float32") + K * U * terms, f"y {kind}")
 
 
+@pytest.mark.parametrize("B,P,C,G", [(2, 300, 64, 8), (2, 40000, 64, 8), (1, 33000, 512, 32), (2, 300, 30, 10)])
+def test_means_whose_square_overflows(sdfl, B, P, C, G):
+    """Around 2^65: the square of a value is no fp32 number, that of a deviation is."""
+    gamma, beta = weights(C, 19)
+    x = (make((B, P, C), "float32", 80).double() * 2.0 ** 53 + 2.0 ** 65).float()
+    y, mean, rstd, _ = sdfl.ops.groupnorm_channels_last_train(x.cuda(), gamma.cuda(), beta.view(1, C).cuda(), G, EPS, False)
+    want, wmean, wrstd, terms = gn_forward(x, gamma, beta, G, EPS, False)
+    size = x.double().abs().reshape(B, P, G, C // G).mean(dim=(1, 3))
+    assert_within(mean, wmean, K * U * size, "mean")
+    assert_within(rstd, wrstd, wrstd * (K * U + (K * U * size * wrstd) ** 2), "rstd")
+    assert_within(y, want, half_step(want, "float32") + K * U * terms, "y")
+    dy = make((B, P, C), "float32", 81)
+    got = sdfl.ops.groupnorm_channels_last_backward(dy.cuda(), x.cuda(), mean, rstd, gamma.cuda(), beta.view(1, C).cuda(), G)
+    assert got[1].shape == (C,) and got[2].shape == (1, C)
+    check_backward((got[0], got[1], got[2].view(C)), dy, x, mean.cpu(), rstd.cpu(), gamma, beta, G, False, "float32", "backward")
+
+
 def test_gradient_against_differences(sdfl):
     B, P, C, G = 2, 30, 24, 6
     x, dy, v = (make((B, P, C), "float32", s) for s in (71, 72, 73))
