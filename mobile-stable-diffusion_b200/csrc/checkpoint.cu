@@ -36,10 +36,14 @@ constexpr int kElemRounds = 2;       // of those, loads first
 
 inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+constexpr int64_t kMaxGridThreads = int64_t{1} << 22;      // of ck_grid
+constexpr int64_t kMaxElementBlocks = kMaxGridThreads / 32 * kElemBlocks * kElemRounds;      // of a round of such a grid
+
 inline unsigned ck_grid(int64_t work_items) {
     int64_t blocks = (work_items + kCkThreads - 1) / kCkThreads;
     const int64_t cap = static_cast<int64_t>(sm_count()) * 8 * 4;
     if (blocks > cap) blocks = cap;
+    if (blocks > kMaxGridThreads / kCkThreads) blocks = kMaxGridThreads / kCkThreads;
     if (blocks < 1) blocks = 1;
     return static_cast<unsigned>(blocks);
 }
@@ -87,32 +91,35 @@ pack_vec_kernel(const uint4 *__restrict__ src, typename CodeVec<VecOf<T>::N>::ty
     }
 }
 
-template <typename T>
+__device__ __forceinline__ int divide(int n, int, const FastDiv &div) { return static_cast<int>(div.div(static_cast<uint32_t>(n))); }
+__device__ __forceinline__ long long divide(long long n, long long by, const FastDiv &) { return n / by; }
+
+template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 pack_element_kernel(const T *__restrict__ src, int8_t *__restrict__ codes, uint8_t *__restrict__ scales,
-                    long long nblocks, long long dim, long long blocks_row, FastDiv row_div, bool narrow) {
+                    I nblocks, I dim, I blocks_row, FastDiv row_div) {
     constexpr uint32_t LANES = kCkptBlock / kElems;
     const uint32_t lane = threadIdx.x & 31;
-    const long long step = static_cast<long long>(kElemBlocks) * kElemRounds;
-    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32) * step;
-    for (long long first = (static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
+    const I step = kElemBlocks * kElemRounds;
+    const I stride = static_cast<I>(gridDim.x) * (kCkThreads / 32) * step;
+    for (I first = (static_cast<I>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
          first < nblocks; first += stride) {
-        long long at[kElemRounds];
+        I at[kElemRounds];
         int left[kElemRounds];                        // of this lane's elements, those inside the row
         float x[kElemRounds][kElems];
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const long long b = first + r * kElemBlocks + lane / LANES;
-            const long long row = narrow ? row_div.div(static_cast<uint32_t>(b)) : b / blocks_row;
-            const long long col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            const I b = first + r * kElemBlocks + lane / LANES;
+            const I row = divide(b, blocks_row, row_div);
+            const I col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
             at[r] = row * dim + col;
-            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<long long>(kElems))) : 0;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kElems))) : 0;
 #pragma unroll
             for (int k = 0; k < kElems; ++k) x[r][k] = k < left[r] ? to_float<T>(src[at[r] + k]) : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const long long b = first + r * kElemBlocks + lane / LANES;
+            const I b = first + r * kElemBlocks + lane / LANES;
             const CkptScale s = ckpt_scale(block_lanes_max<kElems>(max_abs_bits<kElems>(x[r])));
 #pragma unroll
             for (int k = 0; k < kElems; ++k)
@@ -122,9 +129,9 @@ pack_element_kernel(const T *__restrict__ src, int8_t *__restrict__ codes, uint8
     }
 }
 
-// Division of a block number by the blocks of a row: multiply-high while the numbers fit 31 bits (with room for
-// the last round's overhang), a 64-bit division beyond.
-inline bool narrow_blocks(int64_t nblocks) { return nblocks + kElemBlocks * kElemRounds < (1ll << 31); }
+// 32-bit indices and a division by multiply-high while all elements of the padded rows, and the last round's
+// overhang of every warp, fit 31 bits; 64-bit ones beyond.
+inline bool narrow_blocks(int64_t nblocks) { return (nblocks + kMaxElementBlocks) * kCkptBlock < (1ll << 31); }
 inline unsigned element_grid(int64_t nblocks) { return ck_grid((nblocks + kElemRounds * kElemBlocks - 1) / (kElemRounds * kElemBlocks) * 32); }
 
 template <typename T>
@@ -144,10 +151,13 @@ cudaError_t pack_dispatch(const void *src, int8_t *codes, uint8_t *scales, int64
             static_cast<uint32_t>(slots_row), FastDiv::make(static_cast<uint32_t>(slots_row)),
             static_cast<uint32_t>(dim / VEC));
     } else {
-        const bool narrow = narrow_blocks(nblocks);
-        pack_element_kernel<T><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
-            static_cast<const T *>(src), codes, scales, nblocks, dim, blocks_row,
-            FastDiv::make(narrow ? static_cast<uint32_t>(blocks_row) : 1), narrow);
+        if (narrow_blocks(nblocks))
+            pack_element_kernel<T, int><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+                static_cast<const T *>(src), codes, scales, static_cast<int>(nblocks), static_cast<int>(dim),
+                static_cast<int>(blocks_row), FastDiv::make(static_cast<uint32_t>(blocks_row)));
+        else
+            pack_element_kernel<T, long long><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+                static_cast<const T *>(src), codes, scales, nblocks, dim, blocks_row, FastDiv::make(1));
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
@@ -189,27 +199,27 @@ unpack_vec_kernel(const typename CodeVec<VecOf<T>::N>::type *__restrict__ codes,
     }
 }
 
-template <typename T>
+template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 unpack_element_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales, T *__restrict__ dst,
-                      long long nblocks, long long dim, long long blocks_row, FastDiv row_div, bool narrow) {
+                      I nblocks, I dim, I blocks_row, FastDiv row_div) {
     constexpr uint32_t LANES = kCkptBlock / kElems;
     const uint32_t lane = threadIdx.x & 31;
-    const long long step = static_cast<long long>(kElemBlocks) * kElemRounds;
-    const long long stride = static_cast<long long>(gridDim.x) * (kCkThreads / 32) * step;
-    for (long long first = (static_cast<long long>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
+    const I step = kElemBlocks * kElemRounds;
+    const I stride = static_cast<I>(gridDim.x) * (kCkThreads / 32) * step;
+    for (I first = (static_cast<I>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
          first < nblocks; first += stride) {
-        long long at[kElemRounds];
+        I at[kElemRounds];
         int left[kElemRounds];
         int8_t c[kElemRounds][kElems];
         uint8_t e[kElemRounds];
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const long long b = first + r * kElemBlocks + lane / LANES;
-            const long long row = narrow ? row_div.div(static_cast<uint32_t>(b)) : b / blocks_row;
-            const long long col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            const I b = first + r * kElemBlocks + lane / LANES;
+            const I row = divide(b, blocks_row, row_div);
+            const I col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
             at[r] = row * dim + col;
-            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<long long>(kElems))) : 0;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kElems))) : 0;
             e[r] = b < nblocks ? scales[b] : 0;
 #pragma unroll
             for (int k = 0; k < kElems; ++k) c[r][k] = k < left[r] ? codes[at[r] + k] : 0;
@@ -238,10 +248,13 @@ cudaError_t unpack_dispatch(const int8_t *codes, const uint8_t *scales, void *ds
             reinterpret_cast<const CV *>(codes), scales, static_cast<uint4 *>(dst), nvec, static_cast<uint32_t>(vecs_row),
             FastDiv::make(static_cast<uint32_t>(vecs_row)), static_cast<uint32_t>(blocks_row));
     } else {
-        const bool narrow = narrow_blocks(nblocks);
-        unpack_element_kernel<T><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
-            codes, scales, static_cast<T *>(dst), nblocks, dim, blocks_row,
-            FastDiv::make(narrow ? static_cast<uint32_t>(blocks_row) : 1), narrow);
+        if (narrow_blocks(nblocks))
+            unpack_element_kernel<T, int><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+                codes, scales, static_cast<T *>(dst), static_cast<int>(nblocks), static_cast<int>(dim),
+                static_cast<int>(blocks_row), FastDiv::make(static_cast<uint32_t>(blocks_row)));
+        else
+            unpack_element_kernel<T, long long><<<element_grid(nblocks), kCkThreads, 0, stream>>>(
+                codes, scales, static_cast<T *>(dst), nblocks, dim, blocks_row, FastDiv::make(1));
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
@@ -303,14 +316,17 @@ geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
     }
 }
 
+// 32-bit indices as far as the input's elements and a grid's overhang go.
+inline bool narrow_gate(int64_t rows, int64_t d) { return 2 * rows * d + kMaxGridThreads < (1ll << 31); }
+
 // The gate alone, element by element, for rows that are not whole vectors.
-template <typename T>
+template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
-geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, long long rows, long long d, FastDiv row_div, bool narrow) {
+geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, I rows, I d, FastDiv row_div) {
     constexpr bool HALF = sizeof(T) == 2;
-    const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
-    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const long long r = narrow ? row_div.div(static_cast<uint32_t>(i)) : i / d, j = i - r * d;
+    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads;
+    for (I i = static_cast<I>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
+        const I r = divide(i, d, row_div), j = i - r * d;
         dst[i] = from_float<T>(to_float<T>(ab[r * 2 * d + j]) * gelu_erf<HALF>(to_float<T>(ab[r * 2 * d + d + j])));
     }
 }
@@ -338,9 +354,13 @@ cudaError_t geglu_pack_dispatch(const void *ab, void *dst, int8_t *codes, uint8_
         g_launches.fetch_add(1);
         return pack ? cudaSuccess : pack_dispatch<T>(ab, codes, scales, rows, 2 * d, stream);
     }
-    const bool narrow = rows * d < (1ll << 31);
-    geglu_element_kernel<T><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
-        static_cast<const T *>(ab), static_cast<T *>(dst), rows, d, FastDiv::make(narrow ? static_cast<uint32_t>(d) : 1), narrow);
+    if (narrow_gate(rows, d))
+        geglu_element_kernel<T, int><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+            static_cast<const T *>(ab), static_cast<T *>(dst), static_cast<int>(rows), static_cast<int>(d),
+            FastDiv::make(static_cast<uint32_t>(d)));
+    else
+        geglu_element_kernel<T, long long><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+            static_cast<const T *>(ab), static_cast<T *>(dst), rows, d, FastDiv::make(1));
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     g_launches.fetch_add(1);
@@ -410,15 +430,14 @@ geglu_backward_vec_kernel(const uint4 *ab, const typename CodeVec<VecOf<T>::N>::
     }
 }
 
-template <typename T, bool CKPT>
+template <typename T, bool CKPT, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 geglu_backward_element_kernel(const T *ab, const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                              const T *dy, T *dab, long long rows, long long d, long long blocks_row, FastDiv row_div,
-                              bool narrow) {
+                              const T *dy, T *dab, I rows, I d, I blocks_row, FastDiv row_div) {
     constexpr bool HALF = sizeof(T) == 2;
-    const long long total = rows * d, stride = static_cast<long long>(gridDim.x) * kCkThreads;
-    for (long long i = static_cast<long long>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const long long r = narrow ? row_div.div(static_cast<uint32_t>(i)) : i / d, j = i - r * d, at = r * 2 * d + j;
+    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads;
+    for (I i = static_cast<I>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
+        const I r = divide(i, d, row_div), j = i - r * d, at = r * 2 * d + j;
         float a, g;
         if (CKPT) {
             a = ckpt_value(codes[at], scales[r * blocks_row + j / kCkptBlock]);
@@ -448,10 +467,15 @@ cudaError_t geglu_backward_dispatch(const void *ab, const int8_t *codes, const u
             static_cast<const uint4 *>(ab), reinterpret_cast<const CV *>(codes), scales, static_cast<const uint4 *>(dy),
             static_cast<uint4 *>(dab), nvec, FastDiv::make(dvec), dvec, static_cast<uint32_t>(blocks_row));
     } else {
-        const bool narrow = rows * d < (1ll << 31);
-        geglu_backward_element_kernel<T, CKPT><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
-            static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab), rows, d,
-            blocks_row, FastDiv::make(narrow ? static_cast<uint32_t>(d) : 1), narrow);
+        if (narrow_gate(rows, d))
+            geglu_backward_element_kernel<T, CKPT, int><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+                static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab),
+                static_cast<int>(rows), static_cast<int>(d), static_cast<int>(blocks_row),
+                FastDiv::make(static_cast<uint32_t>(d)));
+        else
+            geglu_backward_element_kernel<T, CKPT, long long><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+                static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab), rows, d,
+                blocks_row, FastDiv::make(1));
     }
     cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) g_launches.fetch_add(1);
