@@ -11,12 +11,15 @@
 // rows that are whole vectors; rows that are not whole blocks are walked as if padded to whole
 // blocks, the lanes beyond the row end idle.  A thread takes kVecs vectors 256 apart, all loads first:
 // with one load in flight per thread the kernels reach 78 % of the copy bandwidth.
-// Element kernels, for everything else: four elements per lane, so that what a block costs once (its row,
-// its scale) is paid by 8 lanes for four blocks at a time; one element per lane was 2.2-2.4 times slower.
+// Element kernels, for everything else: eight lanes share a block, so that what a block costs once (its row,
+// its scale) is paid for four blocks at a time; a lane's four elements are eight apart, so that an access of the warp is
+// four sectors.  ([65536, 1003] bf16, pack and expand: one lane per element 213 and 172 us, four elements in a row per
+// lane 73 and 78, eight apart 71 and 58; aligned vectors shifted into place 89 and 81: the shifts and the ragged ends
+// cost more instructions than they save accesses.  Indices are 32 bits wide where they can be: 64 bits took 89.)
 //
 // Measured (B200, back to back in a captured graph; share of the measured copy bandwidth):
-//   pack    [262144, 320] fp16 41 us (97 %), [32768, 320] bf16 7.2 us, [65536, 1003] bf16 (element kernel) 89 us (35 %)
-//   expand  the same 41 us (97 %), 6.7 us, 78 us (40 %)
+//   pack    [262144, 320] fp16 41 us (97 %), [32768, 320] bf16 7.2 us, [65536, 1003] bf16 (element kernel) 71 us (44 %)
+//   expand  the same 41 us (97 %), 6.6 us, 58 us (53 %)
 //   gate with checkpoint  [65536, 1280] bf16 124 us (85 %), [16384, 1280] fp16 32 us (81 %): bound by the integer
 //           operations of the maxima and the codes beside HBM
 //   gate backward  [65536, 1280] bf16 from the input 131 us (99 %), from a checkpoint 112 us (93 %)
@@ -30,9 +33,8 @@ namespace {
 constexpr int kCkThreads = 256;
 constexpr int kVecs = 4;             // vectors per thread and round: pack, expand
 constexpr int kGateVecs = 2;         // of each half: gate
-constexpr int kElems = 4;            // elements per lane: element kernels of pack and expand
-constexpr int kElemBlocks = 32 * kElems / kCkptBlock;      // blocks of a warp at a time
-constexpr int kElemRounds = 2;       // of those, loads first
+// Element kernels of pack and expand: lanes per block, elements per lane, blocks of a warp, rounds of those.
+constexpr int kLanes = 8, kElems = kCkptBlock / kLanes, kElemBlocks = 32 / kLanes, kElemRounds = 2;
 
 inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -98,33 +100,32 @@ template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 pack_element_kernel(const T *__restrict__ src, int8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                     I nblocks, I dim, I blocks_row, FastDiv row_div) {
-    constexpr uint32_t LANES = kCkptBlock / kElems;
-    const uint32_t lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     const I step = kElemBlocks * kElemRounds;
     const I stride = static_cast<I>(gridDim.x) * (kCkThreads / 32) * step;
     for (I first = (static_cast<I>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
          first < nblocks; first += stride) {
         I at[kElemRounds];
-        int left[kElemRounds];                        // of this lane's elements, those inside the row
+        int left[kElemRounds];                        // elements inside the row from this lane's first on; may be negative
         float x[kElemRounds][kElems];
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const I b = first + r * kElemBlocks + lane / LANES;
+            const I b = first + r * kElemBlocks + lane / kLanes;
             const I row = divide(b, blocks_row, row_div);
-            const I col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            const I col = (b - row * blocks_row) * kCkptBlock + lane % kLanes;
             at[r] = row * dim + col;
-            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kElems))) : 0;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kCkptBlock))) : 0;
 #pragma unroll
-            for (int k = 0; k < kElems; ++k) x[r][k] = k < left[r] ? to_float<T>(src[at[r] + k]) : 0.f;
+            for (int k = 0; k < kElems; ++k) x[r][k] = k * kLanes < left[r] ? to_float<T>(src[at[r] + k * kLanes]) : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const I b = first + r * kElemBlocks + lane / LANES;
+            const I b = first + r * kElemBlocks + lane / kLanes;
             const CkptScale s = ckpt_scale(block_lanes_max<kElems>(max_abs_bits<kElems>(x[r])));
 #pragma unroll
             for (int k = 0; k < kElems; ++k)
-                if (k < left[r]) codes[at[r] + k] = static_cast<int8_t>(ckpt_code(x[r][k], s.inv) & s.keep);
-            if (lane % LANES == 0 && b < nblocks) scales[b] = static_cast<uint8_t>(s.e);
+                if (k * kLanes < left[r]) codes[at[r] + k * kLanes] = static_cast<int8_t>(ckpt_code(x[r][k], s.inv) & s.keep);
+            if (lane % kLanes == 0 && b < nblocks) scales[b] = static_cast<uint8_t>(s.e);
         }
     }
 }
@@ -203,8 +204,7 @@ template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 unpack_element_kernel(const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales, T *__restrict__ dst,
                       I nblocks, I dim, I blocks_row, FastDiv row_div) {
-    constexpr uint32_t LANES = kCkptBlock / kElems;
-    const uint32_t lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     const I step = kElemBlocks * kElemRounds;
     const I stride = static_cast<I>(gridDim.x) * (kCkThreads / 32) * step;
     for (I first = (static_cast<I>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5)) * step;
@@ -215,20 +215,20 @@ unpack_element_kernel(const int8_t *__restrict__ codes, const uint8_t *__restric
         uint8_t e[kElemRounds];
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r) {
-            const I b = first + r * kElemBlocks + lane / LANES;
+            const I b = first + r * kElemBlocks + lane / kLanes;
             const I row = divide(b, blocks_row, row_div);
-            const I col = (b - row * blocks_row) * kCkptBlock + (lane % LANES) * kElems;
+            const I col = (b - row * blocks_row) * kCkptBlock + lane % kLanes;
             at[r] = row * dim + col;
-            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kElems))) : 0;
+            left[r] = b < nblocks ? static_cast<int>(min(dim - col, static_cast<I>(kCkptBlock))) : 0;
             e[r] = b < nblocks ? scales[b] : 0;
 #pragma unroll
-            for (int k = 0; k < kElems; ++k) c[r][k] = k < left[r] ? codes[at[r] + k] : 0;
+            for (int k = 0; k < kElems; ++k) c[r][k] = k * kLanes < left[r] ? codes[at[r] + k * kLanes] : 0;
         }
 #pragma unroll
         for (int r = 0; r < kElemRounds; ++r)
 #pragma unroll
             for (int k = 0; k < kElems; ++k)
-                if (k < left[r]) dst[at[r] + k] = from_float<T>(ckpt_value(c[r][k], e[r]));
+                if (k * kLanes < left[r]) dst[at[r] + k * kLanes] = from_float<T>(ckpt_value(c[r][k], e[r]));
     }
 }
 

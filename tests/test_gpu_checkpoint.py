@@ -114,6 +114,40 @@ def test_more_elements_than_31_bits(sdfl):
     assert torch.equal(back[-4:].cpu().double(), values) and int(torch.count_nonzero(back[:-4])) == 0
 
 
+def test_more_elements_than_31_bits_in_odd_rows(sdfl):
+    rows, dim = 70000, 32001
+    x = torch.zeros((rows, dim), dtype=torch.bfloat16, device="cuda")
+    tail = make((4, dim), "bfloat16", 7)
+    x[-4:] = tail.cuda()
+    kept = sdfl.ops.checkpoint_pack(x)
+    codes, scales, values = checkpoint_reference(tail)
+    assert torch.equal(kept.codes[-4:].cpu(), codes) and torch.equal(kept.scales[-4:].cpu(), scales)
+    assert int(torch.count_nonzero(kept.codes[:-4])) == 0
+    del x
+    back = sdfl.ops.checkpoint_unpack(kept)
+    assert torch.equal(back[-4:].cpu().double(), values) and int(torch.count_nonzero(back[:-4])) == 0
+
+
+def test_gate_of_more_elements_than_31_bits_in_odd_rows(sdfl):
+    rows, d = 70000, 16001
+    ab = torch.zeros((rows, 2 * d), dtype=torch.bfloat16, device="cuda")
+    tail = make((4, 2 * d), "bfloat16", 8)
+    ab[-4:] = tail.cuda()
+    y, kept = sdfl.ops.gelu_multiply_checkpoint(ab)
+    _, _, values = checkpoint_reference(tail)
+    want = geglu_forward(tail)
+    assert_within(y[-4:], want, half_step(want, "bfloat16") + geglu_bound(tail, "bfloat16"), "y")
+    assert int(torch.count_nonzero(y[:-4])) == 0
+    y.fill_(0.5)
+    for source, x in ((kept, values), (ab, tail)):
+        got = sdfl.ops.gelu_multiply_backward(y, source, out=ab)
+        want, bound = geglu_backward(torch.full((4, d), 0.5), x, "bfloat16")
+        assert_within(got[-4:], want, half_step(want, "bfloat16") + bound, "gradient")
+        assert int(torch.count_nonzero(got[:-4])) == 0          # a = g = 0
+        ab.zero_()
+        ab[-4:] = tail.cuda()
+
+
 GATE_SHAPES = [(1, 1), (3, 7), (5, 20), (2, 32), (77, 64), (3, 5, 96), (33, 1000), (128, 1280), (9, 5120)]
 
 
