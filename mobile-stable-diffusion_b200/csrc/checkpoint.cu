@@ -22,7 +22,9 @@
 //   expand  the same 41 us (97 %), 6.6 us, 58 us (53 %)
 //   gate with checkpoint  [65536, 1280] bf16 124 us (85 %), [16384, 1280] fp16 32 us (81 %): bound by the integer
 //           operations of the maxima and the codes beside HBM
-//   gate backward  [65536, 1280] bf16 from the input 131 us (99 %), from a checkpoint 112 us (93 %)
+//   gate backward  [65536, 1280] bf16 from the input 131 us (99 %), from a checkpoint 112 us (93 %); element kernel
+//           [8192, 1003] fp32 27 us (94 %) and 32 us (55 %; one element in flight per thread: 35 and 32), bf16 27 (47 %)
+//           and 29 us (36 %): 2-byte accesses
 #include "ckpt_device.cuh"
 #include "kernels.h"
 
@@ -35,6 +37,7 @@ constexpr int kVecs = 4;             // vectors per thread and round: pack, expa
 constexpr int kGateVecs = 2;         // of each half: gate
 // Element kernels of pack and expand: lanes per block, elements per lane, blocks of a warp, rounds of those.
 constexpr int kLanes = 8, kElems = kCkptBlock / kLanes, kElemBlocks = 32 / kLanes, kElemRounds = 2;
+constexpr int kGateElems = 4;        // per thread and round: element kernels of the gate
 
 inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -317,17 +320,29 @@ geglu_pack_kernel(const uint4 *__restrict__ ab, uint4 *__restrict__ dst,
 }
 
 // 32-bit indices as far as the input's elements and a grid's overhang go.
-inline bool narrow_gate(int64_t rows, int64_t d) { return 2 * rows * d + kMaxGridThreads < (1ll << 31); }
+inline bool narrow_gate(int64_t rows, int64_t d) { return 2 * rows * d + kMaxGridThreads * kGateElems < (1ll << 31); }
 
 // The gate alone, element by element, for rows that are not whole vectors.
 template <typename T, typename I>
 __global__ void __launch_bounds__(kCkThreads)
 geglu_element_kernel(const T *__restrict__ ab, T *__restrict__ dst, I rows, I d, FastDiv row_div) {
     constexpr bool HALF = sizeof(T) == 2;
-    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads;
-    for (I i = static_cast<I>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const I r = divide(i, d, row_div), j = i - r * d;
-        dst[i] = from_float<T>(to_float<T>(ab[r * 2 * d + j]) * gelu_erf<HALF>(to_float<T>(ab[r * 2 * d + d + j])));
+    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads * kGateElems;
+    for (I base = static_cast<I>(blockIdx.x) * kCkThreads * kGateElems + threadIdx.x; base < total; base += stride) {
+        float a[kGateElems], g[kGateElems];
+#pragma unroll
+        for (int k = 0; k < kGateElems; ++k) {
+            const I i = base + k * kCkThreads;
+            if (i >= total) continue;
+            const I at = i + divide(i, d, row_div) * d;           // r * 2 d + j
+            a[k] = to_float<T>(ab[at]);
+            g[k] = to_float<T>(ab[at + d]);
+        }
+#pragma unroll
+        for (int k = 0; k < kGateElems; ++k) {
+            const I i = base + k * kCkThreads;
+            if (i < total) dst[i] = from_float<T>(a[k] * gelu_erf<HALF>(g[k]));
+        }
     }
 }
 
@@ -355,11 +370,11 @@ cudaError_t geglu_pack_dispatch(const void *ab, void *dst, int8_t *codes, uint8_
         return pack ? cudaSuccess : pack_dispatch<T>(ab, codes, scales, rows, 2 * d, stream);
     }
     if (narrow_gate(rows, d))
-        geglu_element_kernel<T, int><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+        geglu_element_kernel<T, int><<<ck_grid((rows * d + kGateElems - 1) / kGateElems), kCkThreads, 0, stream>>>(
             static_cast<const T *>(ab), static_cast<T *>(dst), static_cast<int>(rows), static_cast<int>(d),
             FastDiv::make(static_cast<uint32_t>(d)));
     else
-        geglu_element_kernel<T, long long><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+        geglu_element_kernel<T, long long><<<ck_grid((rows * d + kGateElems - 1) / kGateElems), kCkThreads, 0, stream>>>(
             static_cast<const T *>(ab), static_cast<T *>(dst), rows, d, FastDiv::make(1));
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
@@ -435,22 +450,33 @@ __global__ void __launch_bounds__(kCkThreads)
 geglu_backward_element_kernel(const T *ab, const int8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                               const T *dy, T *dab, I rows, I d, I blocks_row, FastDiv row_div) {
     constexpr bool HALF = sizeof(T) == 2;
-    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads;
-    for (I i = static_cast<I>(blockIdx.x) * kCkThreads + threadIdx.x; i < total; i += stride) {
-        const I r = divide(i, d, row_div), j = i - r * d, at = r * 2 * d + j;
-        float a, g;
-        if (CKPT) {
-            a = ckpt_value(codes[at], scales[r * blocks_row + j / kCkptBlock]);
-            g = ckpt_value(codes[at + d], scales[r * blocks_row + (j + d) / kCkptBlock]);
-        } else {
-            a = to_float<T>(ab[at]);
-            g = to_float<T>(ab[at + d]);
+    const I total = rows * d, stride = static_cast<I>(gridDim.x) * kCkThreads * kGateElems;
+    for (I base = static_cast<I>(blockIdx.x) * kCkThreads * kGateElems + threadIdx.x; base < total; base += stride) {
+        I at[kGateElems];
+        float a[kGateElems], g[kGateElems], grad[kGateElems];
+#pragma unroll
+        for (int k = 0; k < kGateElems; ++k) {
+            const I i = base + k * kCkThreads;
+            if (i >= total) continue;
+            const I r = divide(i, d, row_div), j = i - r * d;
+            at[k] = r * 2 * d + j;
+            if (CKPT) {
+                a[k] = ckpt_value(codes[at[k]], scales[r * blocks_row + j / kCkptBlock]);
+                g[k] = ckpt_value(codes[at[k] + d], scales[r * blocks_row + (j + d) / kCkptBlock]);
+            } else {
+                a[k] = to_float<T>(ab[at[k]]);
+                g[k] = to_float<T>(ab[at[k] + d]);
+            }
+            grad[k] = to_float<T>(dy[i]);
         }
-        const float dyi = to_float<T>(dy[i]);
-        float value, slope;
-        gelu_grad<HALF>(g, &value, &slope);
-        dab[at] = from_float<T>(dyi * value);
-        dab[at + d] = from_float<T>(dyi * a * slope);
+#pragma unroll
+        for (int k = 0; k < kGateElems; ++k) {
+            if (base + k * kCkThreads >= total) continue;
+            float value, slope;
+            gelu_grad<HALF>(g[k], &value, &slope);
+            dab[at[k]] = from_float<T>(grad[k] * value);
+            dab[at[k] + d] = from_float<T>(grad[k] * a[k] * slope);
+        }
     }
 }
 
@@ -468,12 +494,12 @@ cudaError_t geglu_backward_dispatch(const void *ab, const int8_t *codes, const u
             static_cast<uint4 *>(dab), nvec, FastDiv::make(dvec), dvec, static_cast<uint32_t>(blocks_row));
     } else {
         if (narrow_gate(rows, d))
-            geglu_backward_element_kernel<T, CKPT, int><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+            geglu_backward_element_kernel<T, CKPT, int><<<ck_grid((rows * d + kGateElems - 1) / kGateElems), kCkThreads, 0, stream>>>(
                 static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab),
                 static_cast<int>(rows), static_cast<int>(d), static_cast<int>(blocks_row),
                 FastDiv::make(static_cast<uint32_t>(d)));
         else
-            geglu_backward_element_kernel<T, CKPT, long long><<<ck_grid(rows * d), kCkThreads, 0, stream>>>(
+            geglu_backward_element_kernel<T, CKPT, long long><<<ck_grid((rows * d + kGateElems - 1) / kGateElems), kCkThreads, 0, stream>>>(
                 static_cast<const T *>(ab), codes, scales, static_cast<const T *>(dy), static_cast<T *>(dab), rows, d,
                 blocks_row, FastDiv::make(1));
     }
