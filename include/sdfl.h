@@ -350,6 +350,8 @@ int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtyp
  *
  * No counterpart in the reference (an inference app on NCHW buffers).  dtype here may also be
  * SDFL_BF16; arithmetic, weights, statistics and weight gradients are fp32.
+ * SiLU here, as in the other entry points, takes the exponential and the reciprocal from the SFU (relative
+ * error about 2^-22 each), down to z = -87; below that its sigmoid is 0.
  *
  * Checkpoint format.  A tensor is seen as [rows, dim]; a row is cut into blocks of 32 consecutive
  * elements, the last one of a row possibly shorter.  With a = max |x| of a block and

@@ -380,7 +380,9 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
 // with P the mean of the thread in row 0: P is close to the block's mean (it can be off by an
 // outlier's share of one thread's pixels, which costs at most log2(rows) bits), so the one
 // subtraction that is left, of N (block mean - P)^2, cancels next to nothing.
-template <typename T, int ACT, bool PACK, bool CLUSTER>
+//
+// SHARE: pairs of elements may share a reciprocal (act_value_half).
+template <typename T, int ACT, bool PACK, bool CLUSTER, bool SHARE>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) {
     constexpr int VEC = VecOf<T>::N;
@@ -616,7 +618,10 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
                 quad_load(cp + col + 4 * h, p);
                 quad_load(cq + col + 4 * h, q);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) e[i] = act_value<ACT>(vfma(vadd(e[i], np), p[i], q[i]));
+                for (int i = 0; i < 2; ++i) {
+                    const Pair z = vfma(vadd(e[i], np), p[i], q[i]);
+                    e[i] = SHARE ? act_value_half<ACT>(z) : act_value<ACT>(z);
+                }
                 half_pack<T>(r, h, e);
             }
             st_stream(o, r);
@@ -1086,16 +1091,23 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
     return err;
 }
 
-template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+template <typename T, bool CLUSTER, bool SHARE> cudaError_t forward_run(const GnClShape &s, Args &a, cudaStream_t stream) {
     CUtensorMap x;
     const cudaError_t err = make_map(&x, a.f.in, s.batch * s.hw, s.channels * sizeof(T), a.p.cols * 16, a.chunk_rows);
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, false, false);
     if (s.act == kActSilu)
-        return a.f.codes ? launch<cl_team_forward_kernel<T, kActSilu, true, CLUSTER>>(a, smem, stream, x)
-                         : launch<cl_team_forward_kernel<T, kActSilu, false, CLUSTER>>(a, smem, stream, x);
-    return a.f.codes ? launch<cl_team_forward_kernel<T, kActNone, true, CLUSTER>>(a, smem, stream, x)
-                     : launch<cl_team_forward_kernel<T, kActNone, false, CLUSTER>>(a, smem, stream, x);
+        return a.f.codes ? launch<cl_team_forward_kernel<T, kActSilu, true, CLUSTER, SHARE>>(a, smem, stream, x)
+                         : launch<cl_team_forward_kernel<T, kActSilu, false, CLUSTER, SHARE>>(a, smem, stream, x);
+    return a.f.codes ? launch<cl_team_forward_kernel<T, kActNone, true, CLUSTER, SHARE>>(a, smem, stream, x)
+                     : launch<cl_team_forward_kernel<T, kActNone, false, CLUSTER, SHARE>>(a, smem, stream, x);
+}
+
+// Clusters are bound by latency, so their kernels have one form.
+template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+    if constexpr (std::is_same_v<T, __half> && !CLUSTER)
+        if (a.width % 2 == 0) return forward_run<T, CLUSTER, true>(s, a, stream);
+    return forward_run<T, CLUSTER, false>(s, a, stream);
 }
 
 template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
