@@ -135,10 +135,17 @@ __device__ __forceinline__ Where locate(const Geometry &g, int64_t hw) {
     return w;
 }
 
-// partial[image][split][channel] = (mean, M2) over the split's pixels
+// What a group's means are counted from: its first value in the image.  Means that lie far from zero would be rounded
+// at their own magnitude, and their differences, which enter the variance, by as much.
+template <typename T>
+__device__ __forceinline__ float group_origin(const T *x, int64_t image, int64_t group, int64_t hw, int64_t channels, int64_t width) {
+    return to_float<T>(x[image * hw * channels + group * width]);
+}
+
+// partial[image][split][channel] = (mean - origin of the group, M2) over the split's pixels
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
-cl_moments_kernel(const T *x, float2 *partial, Geometry g, int64_t hw, int64_t channels) {
+cl_moments_kernel(const T *x, float2 *partial, Geometry g, int64_t hw, int64_t channels, int64_t width) {
     __shared__ float buf[kThreads * VEC];
     __shared__ float mean[kThreads * VEC];
     const Where w = locate(g, hw);
@@ -152,6 +159,9 @@ cl_moments_kernel(const T *x, float2 *partial, Geometry g, int64_t hw, int64_t c
             if (n == 0) m.first(f);
             m.add(f);
         }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            m.k[i] = n > 0 ? m.k[i] - group_origin(x, w.image, (w.channel + i) / width, hw, channels, width) : 0.f;
     }
     const int ncols = g.cols * VEC;
     block_moments<VEC>(m, static_cast<float>(n), w.active || w.row < g.rows, w.row, g.rows, w.col, ncols,
@@ -163,8 +173,9 @@ cl_moments_kernel(const T *x, float2 *partial, Geometry g, int64_t hw, int64_t c
 }
 
 // One block per (image, group): merge of the splits' and channels' moments.
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
-cl_statistics_kernel(const float2 *partial, float2 *stats, float *mean_out, float *rstd_out, int splits, int64_t hw,
+cl_statistics_kernel(const T *x, const float2 *partial, float2 *stats, float *mean_out, float *rstd_out, int splits, int64_t hw,
                      int64_t channels, int64_t groups, float eps) {
     __shared__ float scratch[33];
     const int64_t image = blockIdx.x / groups, group = blockIdx.x % groups;
@@ -188,9 +199,10 @@ cl_statistics_kernel(const float2 *partial, float2 *stats, float *mean_out, floa
     }
     m2 = block_sum(m2, scratch);
     if (threadIdx.x == 0) {
+        const float mu = group_origin(x, image, group, hw, channels, width) + mean;
         const float rstd = 1.0f / sqrtf(m2 / total + eps);
-        stats[blockIdx.x] = make_float2(mean, rstd);
-        if (mean_out) { mean_out[blockIdx.x] = mean; rstd_out[blockIdx.x] = rstd; }
+        stats[blockIdx.x] = make_float2(mu, rstd);
+        if (mean_out) { mean_out[blockIdx.x] = mu; rstd_out[blockIdx.x] = rstd; }
     }
 }
 
@@ -366,9 +378,9 @@ cudaError_t forward_run(const GnClShape &s, const GnClForward &a, void *ws, cuda
     float2 *partial = stats + s.batch * s.groups;
     const T *x = static_cast<const T *>(a.in);
     T *y = static_cast<T *>(a.out);
-    cl_moments_kernel<T, VEC><<<grid, kThreads, 0, stream>>>(x, partial, g, s.hw, s.channels);
-    cl_statistics_kernel<<<static_cast<unsigned>(s.batch * s.groups), kThreads, 0, stream>>>(
-        partial, stats, a.mean, a.rstd, g.splits, s.hw, s.channels, s.groups, s.eps);
+    cl_moments_kernel<T, VEC><<<grid, kThreads, 0, stream>>>(x, partial, g, s.hw, s.channels, s.channels / s.groups);
+    cl_statistics_kernel<T><<<static_cast<unsigned>(s.batch * s.groups), kThreads, 0, stream>>>(
+        x, partial, stats, a.mean, a.rstd, g.splits, s.hw, s.channels, s.groups, s.eps);
     if (s.act == kActSilu)
         cl_normalise_kernel<T, VEC, kActSilu><<<grid, kThreads, 0, stream>>>(x, y, stats, a.gamma, a.beta, g, s.hw,
                                                                             s.channels, s.groups);

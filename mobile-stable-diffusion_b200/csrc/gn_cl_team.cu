@@ -494,19 +494,24 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
         });
         // block sums
         const float n = static_cast<float>(mine), inv = mine ? 1.0f / n : 0.f;
-        float mean[VEC], m2[VEC];
+        float k[VEC], mean[VEC], m2[VEC];             // minus the first value; the mean from there on
+        nk.get(k);
         {
-            float k[VEC], t[VEC], u[VEC];
-            nk.get(k), s.get(t), q.get(u);
+            float t[VEC], u[VEC];
+            s.get(t), q.get(u);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float shift = t[i] * inv;
-                mean[i] = shift - k[i];
-                m2[i] = fmaxf(fmaf(-t[i], shift, u[i]), 0.f);
+                mean[i] = t[i] * inv;
+                m2[i] = fmaxf(fmaf(-t[i], mean[i], u[i]), 0.f);
             }
         }
         block_sync();                              // the buffers may still be read by the pass before
-        if (w.row == 0) shared_store<VEC>(cp + w.col * VEC, mean);
+        if (w.row == 0) {
+            float head[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) head[i] = mean[i] - k[i];
+            shared_store<VEC>(cp + w.col * VEC, head);
+        }
         block_sync();
         if (w.active) {
             float *to = buf + w.row * 2 * w.ncols + w.col * VEC;
@@ -514,7 +519,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
             shared_load<VEC>(cp + w.col * VEC, head);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float d = mine ? mean[i] - head[i] : 0.f;
+                const float d = mine ? mean[i] - (k[i] + head[i]) : 0.f;       // never rounded at the mean's magnitude
                 mean[i] = n * d;
                 m2[i] = mine ? fmaf(n * d, d, m2[i]) : 0.f;
             }
