@@ -75,18 +75,19 @@ __device__ __forceinline__ void block_moments(const ColumnMoments<VEC> &m, float
 }
 
 // ---- per-channel arithmetic ------------------------------------------------------------------------
-// z = (x - pivot) p + q with the mean of the column's first channel as the pivot: where the mean is
-// far from zero compared with the spread, x - pivot loses nothing, and one register serves the vector.
+// z = (x - mean) p + beta with the mean of the channel's own group: where it is far from zero compared with the
+// spread, x - mean loses nothing, and a group's results do not depend on the other groups of its vectors.
 template <int VEC, int ACT> struct Normalise {
-    float pivot, p[VEC], q[VEC];
-    __device__ __forceinline__ void set(int i, float mean, float rstd, float w, float b) {
+    float mean[VEC], p[VEC], q[VEC];
+    __device__ __forceinline__ void set(int i, float mu, float rstd, float w, float b) {
+        mean[i] = mu;
         p[i] = w * rstd;
-        q[i] = fmaf(pivot - mean, p[i], b);
+        q[i] = b;
     }
     __device__ __forceinline__ void apply(float (&f)[VEC]) const {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float z = fmaf(f[i] - pivot, p[i], q[i]);
+            const float z = fmaf(f[i] - mean[i], p[i], q[i]);
             f[i] = act_value<ACT>(z);
         }
     }
@@ -214,7 +215,6 @@ cl_normalise_kernel(const T *x, T *y, const float2 *__restrict__ stats, const fl
     if (!w.active) return;
     const int width = static_cast<int>(channels / groups);
     Normalise<VEC, ACT> a;
-    a.pivot = stats[w.image * groups + w.channel / width].x;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const float2 st = stats[w.image * groups + (w.channel + i) / width];

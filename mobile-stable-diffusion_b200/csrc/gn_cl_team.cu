@@ -374,6 +374,35 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
     block_sync();
 }
 
+// ---- coefficients of a channel, and which channels share a mean ----------------------------------------
+// z = (x - mean) p + beta: where the mean is far from zero compared with the spread, x - mean loses nothing.  It has to
+// be the mean of the channel's own group: around a neighbour's, x would be rounded at that group's distance, and an
+// infinity or a NaN there would reach this one.  Where groups are whole halves of vectors (four channels), the means
+// of a column sit in registers; elsewhere they are read from shared memory like p and beta.
+// ([4, 65536, 320] bf16 forward, ten channels to a group: 96 us, and 94 around one mean per vector.)
+enum Span : int { kHalvesWhole, kPairsWhole, kAnyChannel };
+
+// Where an array of coefficients keeps channel c of a slice: all first halves of the columns, then all second halves, so
+// that neighbouring lanes read neighbouring 16 bytes (32 apart they meet in the banks: [4, 65536, 320] bf16 backward 181 us
+// instead of 165).
+template <int VEC> __device__ __forceinline__ int coef_slot(int c, int cols) {
+    return VEC == 4 ? c : ((c >> 2) & 1) * 4 * cols + (c >> 3) * 4 + (c & 3);
+}
+
+template <typename T, int SPAN> struct Means {
+    static constexpr int N = SPAN == kHalvesWhole ? VecOf<T>::N / 4 : 0;
+    Pair held[N > 0 ? N : 1];
+    // at: minus the means of the first half of this thread's column; `half` floats further on those of the second
+    __device__ __forceinline__ explicit Means(const float *at, int half) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) held[i] = pair(at[i * half], at[i * half]);
+    }
+    __device__ __forceinline__ void get(const float *at, int half, int h, Pair (&m)[2]) const {
+        if constexpr (N > 0) m[0] = m[1] = held[h];
+        else quad_load(at + h * half, m);
+    }
+};
+
 // ---- forward --------------------------------------------------------------------------------------
 // Statistics of a block: every thread keeps sums of d = x - (its first value) and of d^2 per channel and
 // turns them into a mean and a sum of squared deviations.  The block adds up n (mean - P) and M2 + n (mean - P)^2
@@ -381,8 +410,8 @@ __device__ __forceinline__ void sum_rows(float *buf, int rows, int ncols) {
 // outlier's share of one thread's pixels, which costs at most log2(rows) bits), so the one
 // subtraction that is left, of N (block mean - P)^2, cancels next to nothing.
 //
-// SHARE: pairs of elements may share a reciprocal (act_value_half).
-template <typename T, int ACT, bool PACK, bool CLUSTER, bool SHARE>
+// SPAN: what may lie in several groups (below).
+template <typename T, int ACT, bool PACK, bool CLUSTER, int SPAN>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) {
     constexpr int VEC = VecOf<T>::N;
@@ -392,10 +421,10 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     __shared__ uint64_t bars[2 * kStages];
     const Place w = place(a);
     float *buf = reinterpret_cast<float *>(shared + kStages * kChunkBytes);              // [rows][2 ncols]
-    float *cp = buf + 2 * kThreads * VEC;             // [ncols] each: P, later the scale; shift; minus the pivots
+    float *cp = buf + 2 * kThreads * VEC;             // [ncols] each: P, later the scale; beta; minus the means
     float *cq = cp + w.ncols;
-    float *pivots = cq + w.ncols;
-    float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (mean, rstd)
+    float *means = cq + w.ncols;
+    float2 *stat = reinterpret_cast<float2 *>(means + w.ncols);                         // [groups]: (mean, rstd)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     float2 *own = reinterpret_cast<float2 *>(group_of + w.ncols);                        // cluster: [groups], then
     ClusterExchange cluster;                                                             // [groups][members]
@@ -556,8 +585,6 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
         }
     };
 
-    // z = (x - pivot) p + q, the pivot being the mean of the column's first channel: where the mean is far
-    // from zero compared with the spread, x - pivot loses nothing, and one register serves the vector.
     auto apply = [&](int slice, int64_t image) {
         if constexpr (CLUSTER) cluster.wait();
         else wait_all(a, image * a.p.slices + slice, ring.patience);
@@ -604,28 +631,28 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
             const int channel = slice * w.ncols + c;
             const float2 st = stat[group_of[c]];
-            const float pivot = stat[group_of[c - c % VEC]].x;
-            const float scale = a.f.gamma[channel] * st.y;
-            cp[c] = scale;
-            cq[c] = fmaf(pivot - st.x, scale, a.f.beta[channel]);
-            pivots[c] = -pivot;
+            const int at = coef_slot<VEC>(c, a.p.cols);
+            cp[at] = a.f.gamma[channel] * st.y;
+            cq[at] = a.f.beta[channel];
+            means[at] = -st.x;
         }
         block_sync();
-        const int col = w.active ? w.col * VEC : 0;
-        const Pair np = Col::all(pivots[col]);
+        const int col = w.active ? w.col * 4 : 0, half = 4 * a.p.cols;
+        const Means<T, SPAN> minus_means(means + col, half);
         T *o = y + image * a.hw * a.channels + slice * w.ncols + mine0;
         each(resident, [&](const uint4 &v) {
             uint4 r;
 #pragma unroll
             for (int h = 0; h < VEC / 4; ++h) {
-                Pair e[2], p[2], q[2];
+                Pair e[2], p[2], q[2], m[2];
                 half_column<T>(v, h, e);
-                quad_load(cp + col + 4 * h, p);
-                quad_load(cq + col + 4 * h, q);
+                minus_means.get(means + col, half, h, m);
+                quad_load(cp + col + h * half, p);
+                quad_load(cq + col + h * half, q);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const Pair z = vfma(vadd(e[i], np), p[i], q[i]);
-                    e[i] = SHARE ? act_value_half<ACT>(z) : act_value<ACT>(z);
+                    const Pair z = vfma(vadd(e[i], m[i]), p[i], q[i]);
+                    e[i] = std::is_same_v<T, __half> && SPAN < kAnyChannel ? act_value_half<ACT>(z) : act_value<ACT>(z);
                 }
                 half_pack<T>(r, h, e);
             }
@@ -641,7 +668,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
 }
 
 // ---- backward -------------------------------------------------------------------------------------
-template <typename T, int ACT, bool CKPT, bool CLUSTER>
+template <typename T, int ACT, bool CKPT, bool CLUSTER, int SPAN>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
 cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy) {
     constexpr int VEC = VecOf<T>::N;
@@ -656,12 +683,12 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     const Place w = place(a);
     float *buf = reinterpret_cast<float *>(shared + kStagesGrad * kChunkBytes);          // [rows][2 ncols]
     float *total = buf + 2 * kThreads * VEC;          // [2 ncols]: this slice's channel sums over the images
-    float *cp = total + 2 * w.ncols;                  // [ncols] each: scale and shift of z; c0 and c1; minus the pivots
+    float *cp = total + 2 * w.ncols;                  // [ncols] each: scale and beta; c0 and c1; minus the means
     float *cq = cp + w.ncols;
     float *c0 = cq + w.ncols;
     float *c1 = c0 + w.ncols;
-    float *pivots = c1 + w.ncols;
-    float2 *stat = reinterpret_cast<float2 *>(pivots + w.ncols);                         // [groups]: (s1, s2)
+    float *means = c1 + w.ncols;
+    float2 *stat = reinterpret_cast<float2 *>(means + w.ncols);                         // [groups]: (s1, s2)
     int *group_of = reinterpret_cast<int *>(stat + w.ncols);                             // [ncols], within a slice
     float2 *own = reinterpret_cast<float2 *>(group_of + w.ncols);                        // cluster: [groups], then
     ClusterExchange cluster;                                                             // [groups][members]
@@ -733,11 +760,13 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             load_scales(mine);
         }
     };
-    // use(h, coefficients, x - pivot, grad_out, vector) for both halves of each of this thread's vectors, then
+    const int col = w.active ? w.col * 4 : 0, half = 4 * a.p.cols;                      // this column's coefficients
+    // use(h, coefficients, x - mean, grad_out, vector) for both halves of each of this thread's vectors, then
     // done(vector).  The coefficients are read from shared memory where they are used: held in
     // registers they would take a third of the warps away.
-    auto each = [&](bool again, Pair np, auto coefficient, auto use, auto done) {
+    auto each = [&](bool again, auto coefficient, auto use, auto done) {
         int left = mine;
+        const Means<T, SPAN> minus_means(means + col, half);
         if (again) ring.rewind();
         for (int c = 0; c < w.chunks; ++c, left -= kRoundsGrad) {
             ring.wait_full();
@@ -752,17 +781,18 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
 #pragma unroll
                 for (int h = 0; h < VEC / 4; ++h) {
                     const auto coef = coefficient(h);
-                    Pair xm[2], g[2];
+                    Pair xm[2], g[2], m[2];
                     half_column<T>(d, h, g);
+                    minus_means.get(means + col, half, h, m);
                     if constexpr (CKPT) {
                         half_codes(v, h, xm);
                         const Pair st = Col::all(ckpt_step(ek));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) xm[i] = vfma(xm[i], st, np);
+                        for (int i = 0; i < 2; ++i) xm[i] = vfma(xm[i], st, m[i]);
                     } else {
                         half_column<T>(v, h, xm);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) xm[i] = vadd(xm[i], np);
+                        for (int i = 0; i < 2; ++i) xm[i] = vadd(xm[i], m[i]);
                     }
                     use(h, coef, xm, g, d);
                 }
@@ -782,22 +812,22 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     };
     struct Coef { Pair p[2], q[2], k0[2], k1[2]; };
 
-    // z = (x - pivot) p + q as in the forward pass
+    // z = (x - mean) p + beta as in the forward pass
     auto coefficients = [&](int slice, int64_t image, bool second) {
         block_sync();                              // the arrays may still be read by the pass before
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
             const int channel = slice * w.ncols + c;
             const int64_t group0 = image * a.groups + slice * w.slice_groups;
             const int64_t st = group0 + group_of[c];
-            const float mean = a.b.mean[st], rs = a.b.rstd[st], pivot = a.b.mean[group0 + group_of[c - c % VEC]];
-            const float scale = a.b.gamma[channel] * rs;
-            cp[c] = scale;
-            cq[c] = fmaf(pivot - mean, scale, a.b.beta[channel]);
-            pivots[c] = -pivot;
+            const float rs = a.b.rstd[st];
+            const int at = coef_slot<VEC>(c, a.p.cols);
+            cp[at] = a.b.gamma[channel] * rs;
+            cq[at] = a.b.beta[channel];
+            means[at] = -a.b.mean[st];
             if (second) {
                 const float2 s = stat[group_of[c]];
-                c1[c] = -rs * rs * s.y;
-                c0[c] = fmaf(pivot - mean, c1[c], -rs * s.x);
+                c1[at] = -rs * rs * s.y;
+                c0[at] = -rs * s.x;
             }
         }
         block_sync();
@@ -809,12 +839,11 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
         Col s0, s1;
 #pragma unroll
         for (int i = 0; i < Col::N; ++i) { s0.e[i] = Col::all(0.f); s1.e[i] = Col::all(0.f); }
-        const int col = w.active ? w.col * VEC : 0;
-        each(false, Col::all(pivots[col]),
+        each(false,
              [&](int h) {
                  Coef c;
-                 quad_load(cp + col + 4 * h, c.p);
-                 quad_load(cq + col + 4 * h, c.q);
+                 quad_load(cp + col + h * half, c.p);
+                 quad_load(cq + col + h * half, c.q);
                  return c;
              },
              [&](int h, const Coef &c, const Pair (&xm)[2], const Pair (&g)[2], uint4 &) {
@@ -834,9 +863,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
         sum_rows(buf, a.p.rows, 2 * w.ncols);
         const int64_t group0 = image * a.groups + slice * w.slice_groups;
         for (int c = threadIdx.x; c < w.ncols; c += kThreads) {
-            const int64_t st = group0 + group_of[c];
-            // from sums around the pivot to sums of dz xhat
-            const float t = fmaf(-pivots[c] - a.b.mean[st], buf[c], buf[w.ncols + c]) * a.b.rstd[st];
+            const float t = buf[w.ncols + c] * a.b.rstd[group0 + group_of[c]];          // sum of dz xhat
             buf[w.ncols + c] = t;
             total[c] += buf[c];
             total[w.ncols + c] += t;
@@ -890,15 +917,14 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
             if (lane == 0) stat[g] = make_float2(t1 * inv, t2 * inv);
         }
         coefficients(slice, image, true);
-        const int col = w.active ? w.col * VEC : 0;
         T *o = dx + image * a.hw * a.channels + slice * w.ncols + mine0;
-        each(resident, Col::all(pivots[col]),
+        each(resident,
              [&](int h) {
                  Coef c;
-                 quad_load(cp + col + 4 * h, c.p);
-                 quad_load(cq + col + 4 * h, c.q);
-                 quad_load(c0 + col + 4 * h, c.k0);
-                 quad_load(c1 + col + 4 * h, c.k1);
+                 quad_load(cp + col + h * half, c.p);
+                 quad_load(cq + col + h * half, c.q);
+                 quad_load(c0 + col + h * half, c.k0);
+                 quad_load(c1 + col + h * half, c.k1);
                  return c;
              },
              [&](int h, const Coef &c, const Pair (&xm)[2], const Pair (&g)[2], uint4 &r) {
@@ -1096,26 +1122,19 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
     return err;
 }
 
-template <typename T, bool CLUSTER, bool SHARE> cudaError_t forward_run(const GnClShape &s, Args &a, cudaStream_t stream) {
+template <typename T, bool CLUSTER, int SPAN> cudaError_t forward_run(const GnClShape &s, Args &a, cudaStream_t stream) {
     CUtensorMap x;
     const cudaError_t err = make_map(&x, a.f.in, s.batch * s.hw, s.channels * sizeof(T), a.p.cols * 16, a.chunk_rows);
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, false, false);
     if (s.act == kActSilu)
-        return a.f.codes ? launch<cl_team_forward_kernel<T, kActSilu, true, CLUSTER, SHARE>>(a, smem, stream, x)
-                         : launch<cl_team_forward_kernel<T, kActSilu, false, CLUSTER, SHARE>>(a, smem, stream, x);
-    return a.f.codes ? launch<cl_team_forward_kernel<T, kActNone, true, CLUSTER, SHARE>>(a, smem, stream, x)
-                     : launch<cl_team_forward_kernel<T, kActNone, false, CLUSTER, SHARE>>(a, smem, stream, x);
+        return a.f.codes ? launch<cl_team_forward_kernel<T, kActSilu, true, CLUSTER, SPAN>>(a, smem, stream, x)
+                         : launch<cl_team_forward_kernel<T, kActSilu, false, CLUSTER, SPAN>>(a, smem, stream, x);
+    return a.f.codes ? launch<cl_team_forward_kernel<T, kActNone, true, CLUSTER, SPAN>>(a, smem, stream, x)
+                     : launch<cl_team_forward_kernel<T, kActNone, false, CLUSTER, SPAN>>(a, smem, stream, x);
 }
 
-// Clusters are bound by latency, so their kernels have one form.
-template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
-    if constexpr (std::is_same_v<T, __half> && !CLUSTER)
-        if (a.width % 2 == 0) return forward_run<T, CLUSTER, true>(s, a, stream);
-    return forward_run<T, CLUSTER, false>(s, a, stream);
-}
-
-template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+template <typename T, bool CLUSTER, int SPAN> cudaError_t backward_run(const GnClShape &s, Args &a, cudaStream_t stream) {
     const int64_t rows = s.batch * s.hw, row_bytes = s.channels * sizeof(T);
     CUtensorMap x, dy;
     cudaError_t err = make_map(&dy, a.b.grad_out, rows, row_bytes, a.p.cols * 16, a.chunk_rows);
@@ -1125,10 +1144,23 @@ template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s
     if (err != cudaSuccess) return err;
     const size_t smem = shared_bytes(a.p, true, a.b.codes != nullptr);
     if (s.act == kActSilu)
-        return a.b.codes ? launch<cl_team_backward_kernel<T, kActSilu, true, CLUSTER>>(a, smem, stream, x, dy)
-                         : launch<cl_team_backward_kernel<T, kActSilu, false, CLUSTER>>(a, smem, stream, x, dy);
-    return a.b.codes ? launch<cl_team_backward_kernel<T, kActNone, true, CLUSTER>>(a, smem, stream, x, dy)
-                     : launch<cl_team_backward_kernel<T, kActNone, false, CLUSTER>>(a, smem, stream, x, dy);
+        return a.b.codes ? launch<cl_team_backward_kernel<T, kActSilu, true, CLUSTER, SPAN>>(a, smem, stream, x, dy)
+                         : launch<cl_team_backward_kernel<T, kActSilu, false, CLUSTER, SPAN>>(a, smem, stream, x, dy);
+    return a.b.codes ? launch<cl_team_backward_kernel<T, kActNone, true, CLUSTER, SPAN>>(a, smem, stream, x, dy)
+                     : launch<cl_team_backward_kernel<T, kActNone, false, CLUSTER, SPAN>>(a, smem, stream, x, dy);
+}
+
+// The most special form for the width of a group; only the fp16 forward pass gains from whole pairs.
+template <typename T, bool CLUSTER> cudaError_t forward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+    if (a.width % 4 == 0) return forward_run<T, CLUSTER, kHalvesWhole>(s, a, stream);
+    if constexpr (std::is_same_v<T, __half>)
+        if (a.width % 2 == 0) return forward_run<T, CLUSTER, kPairsWhole>(s, a, stream);
+    return forward_run<T, CLUSTER, kAnyChannel>(s, a, stream);
+}
+
+template <typename T, bool CLUSTER> cudaError_t backward_type(const GnClShape &s, Args &a, cudaStream_t stream) {
+    if (a.width % 4 == 0) return backward_run<T, CLUSTER, kHalvesWhole>(s, a, stream);
+    return backward_run<T, CLUSTER, kAnyChannel>(s, a, stream);
 }
 
 }  // namespace
