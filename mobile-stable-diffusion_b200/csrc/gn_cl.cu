@@ -66,11 +66,24 @@ size_t gn_cl_workspace_bytes(const GnClShape &s, bool backward) {
     return bytes;
 }
 
+// Teams need all of their blocks on the device at once; where it has no room for them, several launches do the same.
+namespace {
+
+bool no_room(cudaError_t err) {
+    if (err != cudaErrorCooperativeLaunchTooLarge) return false;
+    (void)cudaGetLastError();
+    return true;
+}
+
+}  // namespace
+
 cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void *ws, cudaStream_t stream) {
     const bool vectors = vectors_ok(a.in, a.out, nullptr);
     GnClTeamPlan p;
-    if (a.codes && vectors && aligned(a.codes, s.dtype == kF32 ? 4 : 8) && find_plan(s, true, false, false, &p))
-        return gn_cl_team_forward(s, p, a, ws, stream);
+    if (a.codes && vectors && aligned(a.codes, s.dtype == kF32 ? 4 : 8) && find_plan(s, true, false, false, &p)) {
+        const cudaError_t err = gn_cl_team_forward(s, p, a, ws, stream);
+        if (!no_room(err)) return err;
+    }
     GnClForward norm = a;
     if (a.codes) {                                     // two steps, the checkpoint first: out may be in
         const cudaError_t err = ckpt_pack_launch(a.in, a.codes, a.scales, s.batch * s.hw, s.channels, s.dtype, stream);
@@ -78,15 +91,20 @@ cudaError_t gn_cl_forward_launch(const GnClShape &s, const GnClForward &a, void 
         norm.codes = nullptr;
         norm.scales = nullptr;
     }
-    if (vectors && find_plan(s, false, false, false, &p)) return gn_cl_team_forward(s, p, norm, ws, stream);
+    if (vectors && find_plan(s, false, false, false, &p)) {
+        const cudaError_t err = gn_cl_team_forward(s, p, norm, ws, stream);
+        if (!no_room(err)) return err;
+    }
     return gn_cl_split_forward(s, norm, ws, stream);
 }
 
 cudaError_t gn_cl_backward_launch(const GnClShape &s, const GnClBackward &a, void *ws, cudaStream_t stream) {
     GnClTeamPlan p;
     if (vectors_ok(a.in, a.grad_out, a.grad_in) && aligned(a.codes, 16) &&
-        find_plan(s, false, true, a.codes != nullptr, &p))
-        return gn_cl_team_backward(s, p, a, ws, stream);
+        find_plan(s, false, true, a.codes != nullptr, &p)) {
+        const cudaError_t err = gn_cl_team_backward(s, p, a, ws, stream);
+        if (!no_room(err)) return err;
+    }
     return gn_cl_split_backward(s, a, ws, stream);
 }
 

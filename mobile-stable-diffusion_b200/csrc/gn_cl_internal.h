@@ -28,6 +28,7 @@ struct GnClTeamPlan {
 // false: no plan for this shape.  pack: the forward pass also writes a checkpoint; ckpt: the
 // backward pass reads one.
 bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, GnClTeamPlan *p);
+size_t gn_cl_team_shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt);    // dynamic, of a thread block
 size_t gn_cl_team_workspace_bytes(const GnClShape &s, const GnClTeamPlan &p, bool backward);
 cudaError_t gn_cl_team_forward(const GnClShape &s, const GnClTeamPlan &p, const GnClForward &a, void *ws, cudaStream_t stream);
 cudaError_t gn_cl_team_backward(const GnClShape &s, const GnClTeamPlan &p, const GnClBackward &a, void *ws,

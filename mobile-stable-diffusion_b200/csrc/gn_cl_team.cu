@@ -79,6 +79,8 @@ constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward
 // instead of two: 13 us against 16 when calls are made one by one.  Clusters of 16 start 7 us later.
 constexpr int kMaxCluster = 8;
 constexpr size_t kMaxShared = 200 * 1024;
+constexpr int64_t kSmShared = 228 * 1024;          // of an SM
+constexpr int64_t kBlockShared = 1024 + 128;       // that a block takes besides its dynamic shared memory: reserved, static
 constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
 constexpr int kSlotWords = 1024 + kMaxTeamsOfSm;
@@ -1076,19 +1078,29 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int64_t rows, int64_t r
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Blocks of a kernel that an SM holds; asked once per thread and change of size.
+template <auto kernel> cudaError_t blocks_of_sm(int dev, size_t smem, int *blocks) {
+    struct Known { int dev = -1, blocks = 0; size_t smem = 0; };
+    thread_local Known known;
+    if (known.dev != dev || known.smem != smem) {
+        known.dev = -1;
+        const cudaError_t err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known.blocks, kernel, kBlock, smem);
+        if (err != cudaSuccess) return err;
+        known.dev = dev;
+        known.smem = smem;
+    }
+    *blocks = known.blocks;
+    return cudaSuccess;
+}
+
 // A team is a cluster, or else the launch is cooperative: the blocks of a team wait for one another, so
-// either all of them run or none.
+// either all of them run or none.  A grid that the device does not hold at once is not launched at all
+// (cudaErrorCooperativeLaunchTooLarge): the caller has a form without teams.
 template <auto kernel, typename... Maps>
 cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &...maps) {
     cudaError_t err;
     const bool counted = !a.p.cluster && a.p.members > 1;
-    if (counted) {
-        const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
-        cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
-        err = cudaGetLastError();
-        if (err != cudaSuccess) return err;
-        g_launches.fetch_add(1);
-    }
+    const int grid = a.p.slice_teams * a.p.image_teams * a.p.members;
     // once per kernel and device, to what any of its plans may ask for
     static std::atomic<bool> prepared[kMaxDevices];
     int dev = 0;
@@ -1100,8 +1112,19 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
         if (dev < kMaxDevices) prepared[dev].store(true, std::memory_order_relaxed);
     }
     if (smem > kMaxShared) return cudaErrorInvalidConfiguration;
+    if (counted) {
+        int blocks = 0;
+        err = blocks_of_sm<kernel>(dev, smem, &blocks);
+        if (err != cudaSuccess) return err;
+        if (grid > static_cast<int64_t>(blocks) * sm_count()) return cudaErrorCooperativeLaunchTooLarge;
+        const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
+        cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
+        err = cudaGetLastError();
+        if (err != cudaSuccess) return err;
+        g_launches.fetch_add(1);
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.p.slice_teams * a.p.image_teams * a.p.members));
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kBlock);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -1229,8 +1252,8 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
         if (allowed(d) && (slices == 0 || (grains / d >= want && d * images <= sms * kBlocksPerSm))) slices = d;
     if (slices == 0) return false;
     const int64_t chunks = set_slices(slices);
-    // what an SM holds at once: 228 KB of shared memory, 1 KB of it reserved per block
-    const int64_t fit = 228 * 1024 / (static_cast<int64_t>(shared_bytes(*p, backward, ckpt)) + 1024);
+    // what an SM holds at once
+    const int64_t fit = kSmShared / (static_cast<int64_t>(shared_bytes(*p, backward, ckpt)) + kBlockShared);
     const int64_t blocks = sms * std::min<int64_t>(fit, kBlocksPerSm);
     p->slice_teams = static_cast<int>(std::min(slices, std::max<int64_t>(1, in_flight * slices / image)));
     while (slices % p->slice_teams != 0) --p->slice_teams;
@@ -1242,6 +1265,8 @@ bool gn_cl_team_plan(const GnClShape &s, bool pack, bool backward, bool ckpt, Gn
     p->stagger = !p->resident && p->slice_teams * n == kMaxTeamsOfSm && p->members == sms && fit >= kBlocksPerSm;
     return true;
 }
+
+size_t gn_cl_team_shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt) { return shared_bytes(p, backward, ckpt); }
 
 size_t gn_cl_team_workspace_bytes(const GnClShape &s, const GnClTeamPlan &p, bool backward) {
     return layout(s, p, backward).bytes;
