@@ -80,6 +80,7 @@ constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward
 constexpr int kMaxCluster = 8;
 constexpr size_t kMaxShared = 200 * 1024;
 constexpr int64_t kSmShared = 228 * 1024;          // of an SM
+constexpr size_t kTwoOnSm = kSmShared / 3;          // staggered teams number their blocks by two on every SM: a third has no room
 constexpr int64_t kBlockShared = 1024 + 128;       // that a block takes besides its dynamic shared memory: reserved, static
 constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
@@ -1041,9 +1042,10 @@ Args make_args(const GnClShape &s, const GnClTeamPlan &p, bool backward, void *w
 size_t shared_bytes(const GnClTeamPlan &p, bool backward, bool ckpt) {
     const size_t ncols = static_cast<size_t>(p.cols) * p.vec;
     const size_t vector = !backward ? 16 : ckpt ? 16 + p.vec : 32;
-    return static_cast<size_t>(backward ? stages_grad(ckpt) * rounds_grad(ckpt) : kStages * kRounds) * kThreads * vector +
+    const size_t bytes = static_cast<size_t>(backward ? stages_grad(ckpt) * rounds_grad(ckpt) : kStages * kRounds) * kThreads * vector +
            (2 * static_cast<size_t>(kThreads) * p.vec + (backward ? 10 : 6) * ncols) * sizeof(float) +
            (p.cluster ? static_cast<size_t>(p.slice_groups) * (1 + p.members) * sizeof(float2) : 0);
+    return p.stagger ? std::max(bytes, kTwoOnSm) : bytes;
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -1116,7 +1118,7 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
         int blocks = 0;
         err = blocks_of_sm<kernel>(dev, smem, &blocks);
         if (err != cudaSuccess) return err;
-        if (grid > static_cast<int64_t>(blocks) * sm_count()) return cudaErrorCooperativeLaunchTooLarge;
+        if (grid > static_cast<int64_t>(blocks) * sm_count() || (a.p.stagger && blocks != kMaxTeamsOfSm)) return cudaErrorCooperativeLaunchTooLarge;
         const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
         cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
         err = cudaGetLastError();

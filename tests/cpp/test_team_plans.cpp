@@ -1,15 +1,16 @@
 // Plans of the channels-last GroupNorm over a sweep of shapes: the grid of a plan whose blocks wait for one another has
-// to fit the device at once.  Needs no device (148 SMs are assumed without one).  Prints the plans that do not hold.
+// to fit the device at once, and of a staggered plan, whose blocks number themselves by two on every SM, no third block may
+// fit an SM, whatever the kernel's registers.  Needs no device (148 SMs are assumed without one).  Prints the plans that do not hold.
 #include "../../mobile-stable-diffusion_b200/csrc/gn_cl_internal.h"
 
 #include <algorithm>
 #include <cstdio>
 
 // An SM's shared memory, and what a block takes of it: its dynamic part, 128 bytes static (from the compiler's
-// report), 1 KB reserved, in units of 128 bytes.  Registers allow two blocks.
+// report), 1 KB reserved, in units of 128 bytes.
 static int blocks_of_sm(size_t dynamic) {
     const size_t block = (dynamic + 128 + 127) / 128 * 128 + 1024;
-    return static_cast<int>(std::min<size_t>(228 * 1024 / block, 2));
+    return static_cast<int>(228 * 1024 / block);
 }
 
 int main() {
@@ -29,7 +30,7 @@ int main() {
         if (p.cluster || p.members == 1) continue;
         const int fit = blocks_of_sm(gn_cl_team_shared_bytes(p, backward, ckpt));
         const int64_t grid = static_cast<int64_t>(p.slice_teams) * p.image_teams * p.members;
-        if (grid > fit * 148) {
+        if (grid > std::min(fit, 2) * 148 || (p.stagger && fit != 2)) {            // registers allow two blocks
             std::printf("[%lld, %lld, %lld] groups %lld dtype %d kind %d: %lld blocks, %d per SM\n", (long long)b, (long long)hw,
                         (long long)(w * g), (long long)g, dtype, kind, (long long)grid, fit);
             ++wrong;
