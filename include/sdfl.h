@@ -373,7 +373,7 @@ int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtyp
  * workspace: 16-byte aligned, sdfl_groupnorm_channels_last_workspace_bytes(..., backward = 0)
  * bytes, contents of no matter; launches that can overlap on the GPU need one each (two captured
  * graphs that hold the same workspace must not run at the same time).
- * batch == 0 or hw == 0 writes nothing. */
+ * batch == 0 or hw == 0 writes nothing.  The query answers 0 for a shape that the calls refuse. */
 size_t sdfl_groupnorm_channels_last_workspace_bytes(int64_t batch, int64_t channels, int64_t hw,
                                                     int64_t num_groups, int backward, int dtype);
 int sdfl_groupnorm_channels_last_forward(const void *in, void *out, const float *gamma, const float *beta,

@@ -42,15 +42,20 @@ inline bool any_overlap(const void *a, int64_t abytes, const void *b, int64_t bb
     return a0 < b0 + static_cast<uintptr_t>(bbytes) && b0 < a0 + static_cast<uintptr_t>(abytes);
 }
 
+// Sizes that the GroupNorm kernels take, of a shape with positive entries; nothing here overflows, and where it holds
+// the number of elements is below 2^58.
+inline bool gn_size_ok(int64_t batch, int64_t channels, int64_t hw, int64_t groups) {
+    if (hw >= (1ll << 31) || channels >= (1ll << 31) || batch >= (1ll << 27)) return false;
+    return (channels / groups) * hw < (1ll << 31) && batch * groups < (1ll << 27);
+}
+
 int gn_validate(const void *in, const void *out, const float *gamma, const float *beta,
                 int64_t batch, int64_t channels, int64_t hw, int64_t groups, float eps, int dtype) {
     if (!dtype_ok(dtype)) return SDFL_ERR_INVALID_VALUE;
     if (batch < 0 || channels <= 0 || hw < 0 || groups <= 0) return SDFL_ERR_INVALID_VALUE;
     if (channels % groups != 0) return SDFL_ERR_INVALID_VALUE;   // NN/GroupNorm.cpp:83-87
     if (!(eps >= 0.f)) return SDFL_ERR_INVALID_VALUE;
-    if (hw >= (1ll << 31) || channels >= (1ll << 31)) return SDFL_ERR_UNSUPPORTED;
-    if ((channels / groups) * hw >= (1ll << 31)) return SDFL_ERR_UNSUPPORTED;
-    if (batch * groups >= (1ll << 27)) return SDFL_ERR_UNSUPPORTED;
+    if (!gn_size_ok(batch, channels, hw, groups)) return SDFL_ERR_UNSUPPORTED;
     if (batch == 0 || hw == 0) return SDFL_OK;
     if (!in || !out || !gamma || !beta) return SDFL_ERR_INVALID_POINTER;
     const int64_t bytes = batch * channels * hw * esize(dtype);
@@ -97,7 +102,8 @@ inline bool ckpt_overlaps(const void *codes, const void *scales, int64_t rows, i
 }
 inline int ckpt_shape_check(int64_t rows, int64_t dim, int dtype) {
     if (!train_dtype_ok(dtype) || rows < 0 || dim < 0) return SDFL_ERR_INVALID_VALUE;
-    if (dim >= (1ll << 31) || rows >= (1ll << 40)) return SDFL_ERR_UNSUPPORTED;
+    // bytes of twice as many elements (the gate's input) are far from overflowing
+    if (dim >= (1ll << 31) || rows >= (1ll << 40) || (dim > 0 && rows > (1ll << 58) / dim)) return SDFL_ERR_UNSUPPORTED;
     return SDFL_OK;
 }
 
@@ -574,7 +580,7 @@ int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtyp
 size_t sdfl_groupnorm_channels_last_workspace_bytes(int64_t batch, int64_t channels, int64_t hw, int64_t num_groups,
                                                     int backward, int dtype) {
     if (!train_dtype_ok(dtype) || batch <= 0 || channels <= 0 || hw <= 0 || num_groups <= 0 ||
-        channels % num_groups != 0)
+        channels % num_groups != 0 || !gn_size_ok(batch, channels, hw, num_groups))
         return 0;
     sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, 0.f, sdfl::kActNone};
     return sdfl::gn_cl_workspace_bytes(s, backward != 0);
