@@ -366,7 +366,8 @@ int sdfl_elemwise_add(const void *A, const void *B, void *C, int64_t n, int dtyp
 
 /* GroupNorm with optional fused SiLU on a channels-last tensor [batch, hw, channels]: group g of
  * an image is channels [g*C/G, (g+1)*C/G) of all its pixels, biased variance, eps inside the square root, as in
- * sdfl_groupnorm_forward.  out may be in.
+ * sdfl_groupnorm_forward.  out may be in.  Otherwise an array that the call writes (the workspace among them) may touch
+ * no other one (SDFL_ERR_OVERLAP), here and in the backward pass.
  * mean, rstd: NULL, or [batch, num_groups] fp32 that receive the statistics the backward pass
  * needs (rstd = 1 / sqrt(variance + eps)).
  * codes, scales: NULL, or a checkpoint of `in` seen as [batch * hw, channels], written in the same call.

@@ -94,6 +94,19 @@ int gn_cl_validate(const void *in, const void *out, const float *gamma, const fl
                        dtype == SDFL_F32 ? SDFL_F32 : SDFL_F16);
 }
 
+// Arrays of a call, NULL where the call has none.  True if a written one touches another or one that is read.
+struct Array { const void *p; int64_t bytes; };
+inline bool touch(const Array &a, const Array &b) { return a.p && b.p && any_overlap(a.p, a.bytes, b.p, b.bytes); }
+bool arrays_clash(std::initializer_list<Array> written, std::initializer_list<Array> read) {
+    for (const Array *w = written.begin(); w != written.end(); ++w) {
+        for (const Array *v = w + 1; v != written.end(); ++v)
+            if (touch(*w, *v)) return true;
+        for (const Array &r : read)
+            if (touch(*w, r)) return true;
+    }
+    return false;
+}
+
 // A checkpoint's two arrays: both or neither; true if either touches [p, p + bytes).
 inline bool ckpt_half(const void *codes, const void *scales) { return (codes == nullptr) != (scales == nullptr); }
 inline int64_t ckpt_scale_bytes(int64_t rows, int64_t dim) { return rows * ((dim + 31) / 32); }
@@ -594,18 +607,16 @@ int sdfl_groupnorm_channels_last_forward(const void *in, void *out, const float 
     if (rc != SDFL_OK) return rc;
     if (batch == 0 || hw == 0) return SDFL_OK;
     if ((mean == nullptr) != (rstd == nullptr) || ckpt_half(codes, scales)) return SDFL_ERR_INVALID_POINTER;
-    const int64_t bytes = batch * channels * hw * train_esize(dtype), sums = batch * num_groups * 4;
-    if (mean && (any_overlap(mean, sums, out, bytes) || any_overlap(rstd, sums, out, bytes) ||
-                 any_overlap(mean, sums, in, bytes) || any_overlap(rstd, sums, in, bytes) ||
-                 any_overlap(mean, sums, rstd, sums)))
-        return SDFL_ERR_OVERLAP;
-    if (codes && (ckpt_overlaps(codes, scales, batch * hw, channels, in, bytes) ||
-                  ckpt_overlaps(codes, scales, batch * hw, channels, out, bytes) ||
-                  any_overlap(codes, batch * hw * channels, scales, ckpt_scale_bytes(batch * hw, channels))))
-        return SDFL_ERR_OVERLAP;
+    const int64_t bytes = batch * channels * hw * train_esize(dtype), sums = batch * num_groups * 4, params = channels * 4;
+    const Array x{in, bytes}, y{out, bytes}, m{mean, sums}, r{rstd, sums}, w{gamma, params}, b{beta, params},
+        c{codes, batch * hw * channels}, k{scales, ckpt_scale_bytes(batch * hw, channels)};
+    // out may be in, and only that: checked above
+    if (arrays_clash({m, r, c, k}, {x, y, w, b}) || arrays_clash({y}, {w, b})) return SDFL_ERR_OVERLAP;
     sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, eps, fuse_silu ? sdfl::kActSilu : sdfl::kActNone};
-    rc = workspace_check(workspace, workspace_bytes, sdfl::gn_cl_workspace_bytes(s, false));
+    const size_t need = sdfl::gn_cl_workspace_bytes(s, false);
+    rc = workspace_check(workspace, workspace_bytes, need);
     if (rc != SDFL_OK) return rc;
+    if (need && arrays_clash({Array{workspace, static_cast<int64_t>(need)}}, {x, y, m, r, c, k, w, b})) return SDFL_ERR_OVERLAP;
     sdfl::GnClForward a{in, out, gamma, beta, mean, rstd, codes, scales};
     cudaError_t e = sdfl::gn_cl_forward_launch(s, a, workspace, as_stream(stream));
     if (e == cudaErrorInvalidConfiguration) return SDFL_ERR_UNSUPPORTED;
@@ -628,19 +639,20 @@ int sdfl_groupnorm_channels_last_backward(const void *in, const int8_t *codes, c
     }
     if (ckpt_half(codes, scales) || !mean || !rstd || (!in && !codes)) return SDFL_ERR_INVALID_POINTER;
     if (in && codes) return SDFL_ERR_INVALID_VALUE;      // one source
-    const int64_t bytes = batch * channels * hw * train_esize(dtype);
-    if (in && partial_overlap(in, bytes, grad_in, bytes)) return SDFL_ERR_OVERLAP;
-    if (codes && ckpt_overlaps(codes, scales, batch * hw, channels, grad_in, bytes)) return SDFL_ERR_OVERLAP;
-    const int64_t params = channels * 4;
-    for (const float *p : {grad_gamma, grad_beta})
-        if (p && (any_overlap(p, params, grad_in, bytes) || any_overlap(p, params, grad_out, bytes) ||
-                  (in && any_overlap(p, params, in, bytes)) || any_overlap(p, params, gamma, params) ||
-                  any_overlap(p, params, beta, params)))
-            return SDFL_ERR_OVERLAP;
-    if (grad_gamma && grad_beta && any_overlap(grad_gamma, params, grad_beta, params)) return SDFL_ERR_OVERLAP;
+    const int64_t bytes = batch * channels * hw * train_esize(dtype), sums = batch * num_groups * 4, params = channels * 4;
+    const Array x{in, bytes}, dy{grad_out, bytes}, dx{grad_in, bytes}, m{mean, sums}, r{rstd, sums}, w{gamma, params},
+        b{beta, params}, c{codes, batch * hw * channels}, k{scales, ckpt_scale_bytes(batch * hw, channels)},
+        dw{grad_gamma, params}, db{grad_beta, params};
+    // grad_in may be in or grad_out, and only that
+    if ((in && partial_overlap(in, bytes, grad_in, bytes)) || arrays_clash({dx}, {c, k, m, r, w, b}) ||
+        arrays_clash({dw, db}, {dx, dy, x, c, k, m, r, w, b}))
+        return SDFL_ERR_OVERLAP;
     sdfl::GnClShape s{batch, channels, hw, num_groups, dtype, 0.f, fuse_silu ? sdfl::kActSilu : sdfl::kActNone};
-    rc = workspace_check(workspace, workspace_bytes, sdfl::gn_cl_workspace_bytes(s, true));
+    const size_t need = sdfl::gn_cl_workspace_bytes(s, true);
+    rc = workspace_check(workspace, workspace_bytes, need);
     if (rc != SDFL_OK) return rc;
+    if (need && arrays_clash({Array{workspace, static_cast<int64_t>(need)}}, {x, dy, dx, c, k, m, r, w, b, dw, db}))
+        return SDFL_ERR_OVERLAP;
     sdfl::GnClBackward a{in, codes, scales, grad_out, grad_in, gamma, beta, mean, rstd, grad_gamma, grad_beta};
     cudaError_t e = sdfl::gn_cl_backward_launch(s, a, workspace, as_stream(stream));
     if (e == cudaErrorInvalidConfiguration) return SDFL_ERR_UNSUPPORTED;
