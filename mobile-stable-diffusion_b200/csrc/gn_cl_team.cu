@@ -446,7 +446,7 @@ cl_team_forward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x) 
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
             stagger(a, w.team, ring.patience);
-            const uint64_t again = policy_evict_last(), done = policy_evict_first();
+            const uint64_t done = policy_evict_first(), again = resident ? done : policy_evict_last();
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols * sizeof(T));
             while (passes.next(a, w)) {
                 if (passes.second && resident) break;
@@ -710,7 +710,7 @@ cl_team_backward_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
     if (warp == kWarps) {                             // producer
         if (lane == 0) {
             stagger(a, w.team, ring.patience);
-            const uint64_t again = policy_evict_last(), done = policy_evict_first();
+            const uint64_t done = policy_evict_first(), again = resident ? done : policy_evict_last();
             constexpr int kSizeX = CKPT ? 1 : sizeof(T);
             const uint32_t bytes = static_cast<uint32_t>(a.chunk_rows * w.ncols) * (sizeof(T) + kSizeX);
             while (passes.next(a, w)) {
