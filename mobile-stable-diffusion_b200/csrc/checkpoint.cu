@@ -39,8 +39,6 @@ constexpr int kGateVecs = 2;         // of each half: gate
 constexpr int kLanes = 8, kElems = kCkptBlock / kLanes, kElemBlocks = 32 / kLanes, kElemRounds = 2;
 constexpr int kGateElems = 4;        // per thread and round: element kernels of the gate
 
-inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
 constexpr int64_t kMaxGridThreads = int64_t{1} << 22;      // of ck_grid
 constexpr int64_t kMaxElementBlocks = kMaxGridThreads / 32 * kElemBlocks * kElemRounds;      // of a round of such a grid
 

@@ -35,6 +35,8 @@ inline int sm_count() {
     return cached[dev];
 }
 
+inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }      // a: a power of two
+
 // ---------------------------------------------------------------------------------------------
 // 16-byte vectors of T <-> float lanes
 // ---------------------------------------------------------------------------------------------

@@ -9,16 +9,9 @@ namespace sdfl {
 
 namespace {
 
-inline bool aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
 bool vectors_ok(const void *a, const void *b, const void *c) {
     return aligned(a, 16) && aligned(b, 16) && aligned(c, 16);
 }
-
-
-}  // namespace
-
-namespace {
 
 // Plans of recent shapes, per host thread: working one out takes 1-2 us, a tenth of a small call.
 struct PlanKey {

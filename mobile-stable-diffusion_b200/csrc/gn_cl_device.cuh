@@ -3,9 +3,9 @@
 // arithmetic of the normalise and gradient passes.
 //
 // Layout.  [batch, hw, channels]: a pixel is a row of `channels` elements, cut into `columns` of VEC
-// elements.  A thread keeps one column and walks down the rows, so everything that belongs to a
-// channel (weights, statistics, running sums) sits in its registers, and neighbouring threads
-// read neighbouring columns.
+// elements.  A thread keeps one column and walks down the rows, so its channels' running sums sit in its registers
+// and neighbouring threads read neighbouring columns; weights and statistics are read from shared memory
+// (gn_cl_team.cu) or sit in registers too (gn_cl_split.cu).
 //
 //   forward   z = (x - mean) rstd gamma + beta,  y = z or z sigmoid(z)
 //   backward  dz = dy act'(z);  per channel  B = sum dz,  A = sum dz (x - mean)
@@ -22,8 +22,6 @@
 namespace sdfl {
 
 namespace {
-
-inline bool cl_aligned(const void *p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // ---- one column access: VEC elements of one pixel ------------------------------------------------
 template <typename T, int VEC> struct Raw { using type = uint4; };
@@ -212,11 +210,6 @@ template <int VEC> __device__ __forceinline__ void shared_load(const float *from
         }
 }
 
-template <int VEC> __device__ __forceinline__ void column_load(const float *from, Column<VEC> &c) {
-    float f[VEC];
-    shared_load<VEC>(from, f);
-    c.set(f);
-}
 template <int VEC> __device__ __forceinline__ void column_store(float *to, const Column<VEC> &c) {
     float f[VEC];
     c.get(f);

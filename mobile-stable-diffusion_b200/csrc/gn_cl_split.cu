@@ -426,7 +426,7 @@ cudaError_t backward_pick(const GnClShape &s, const GnClBackward &a, void *ws, c
 
 template <typename T> bool vectors_ok(const GnClShape &s, const void *a, const void *b, const void *c, const void *codes) {
     constexpr int VEC = VecOf<T>::N;
-    return s.channels % VEC == 0 && cl_aligned(a, 16) && cl_aligned(b, 16) && cl_aligned(c, 16) && cl_aligned(codes, VEC);
+    return s.channels % VEC == 0 && aligned(a, 16) && aligned(b, 16) && aligned(c, 16) && aligned(codes, VEC);
 }
 
 template <typename T>
