@@ -391,6 +391,7 @@ int sdfl_groupnorm_channels_last_forward(const void *in, void *out, const float 
  *                   over the group's elements
  * grad_gamma and grad_beta are [channels] fp32 and may be NULL; they are written, not added to.
  * Sums run in a fixed order: the same inputs give the same bits.  grad_in may be `in` or grad_out.
+ * rstd^2 is formed in fp32: rstd above 1.8e19 (eps = 0 and a group's values within 1e-19 of one another) overflows.
  * An empty tensor writes zeros to grad_gamma and grad_beta. */
 int sdfl_groupnorm_channels_last_backward(const void *in, const int8_t *codes, const uint8_t *scales,
                                           const void *grad_out, void *grad_in, const float *gamma,

@@ -22,9 +22,8 @@
 //   expand  the same 41 us (97 %), 6.6 us, 58 us (53 %)
 //   gate with checkpoint  [65536, 1280] bf16 124 us (85 %), [16384, 1280] fp16 32 us (81 %): bound by the integer
 //           operations of the maxima and the codes beside HBM
-//   gate backward  [65536, 1280] bf16 from the input 131 us (99 %), from a checkpoint 112 us (93 %); element kernel
-//           [8192, 1003] fp32 27 us (94 %) and 32 us (55 %; one element in flight per thread: 35 and 32), bf16 27 (47 %)
-//           and 29 us (36 %): 2-byte accesses
+//   gate backward  [65536, 1280] bf16 from the input 130 us (100 %), from a checkpoint 112 us (94 %); element kernel
+//           [8192, 1003] fp32 27 us (95 %) and 30 us (60 %), bf16 27 (47 %) and 29 us (36 %): 2-byte accesses
 #include "ckpt_device.cuh"
 #include "kernels.h"
 

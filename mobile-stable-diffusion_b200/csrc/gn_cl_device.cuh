@@ -81,8 +81,8 @@ template <typename T> struct Source<T, 1, true> {
 };
 
 // ---- arithmetic on a column: VEC elements as VEC / 2 pairs ------------------------------------------
-// The packed fp32 instructions (add, mul and fma .f32x2) do two elements per issue slot, and issue slots
-// are what these kernels run short of next to HBM.  VEC = 1 uses the scalar forms.
+// The packed fp32 instructions (add, mul and fma .f32x2) do two elements per instruction; with 16 warps per SM these
+// kernels take about 1.9 cycles per instruction and scheduler.  VEC = 1 uses the scalar forms.
 using Pair = unsigned long long;
 
 __device__ __forceinline__ Pair pair(float lo, float hi) {

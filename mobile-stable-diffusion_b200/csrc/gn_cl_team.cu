@@ -5,14 +5,16 @@
 // checkpoint) and grad_out and one write (backward); but a group's first result needs its last element,
 // so every element is read twice, the second time from shared memory or from L2.  What bounds the
 // forward pass is the sum of the HBM reads of pass S, the L2 reads, arithmetic and stores of pass A and the
-// exchange between them ([4, 262144, 128] fp16 with SiLU: S alone 52 us, 5.1 TB/s; A's loads and the
-// exchange 42; A's arithmetic and stores, which overlap, 40).  The backward pass is bound by issue slots:
-// about 18 instructions per element and pass at 0.56 per cycle and scheduler.
+// exchange between them ([4, 262144, 128] fp16 with SiLU, when it took 134 us: S alone 52 us, 5.1 TB/s; A's loads and the
+// exchange 42; A's arithmetic and stores, which overlap, 40).  The backward pass is bound by latency: about 17
+// instructions per element and pass, of which 16 consumer warps per SM issue 0.53 per cycle and scheduler; the SFU is
+// its busiest pipe (51 %).
 // Measured (B200, back to back in a captured graph; share of the measured copy bandwidth by the bytes above):
-//   forward   [4, 262144, 128] fp16 SiLU 128 us (65 %), [8, 4096, 512] fp16 26 us (41 %), [3, 2961, 640] fp32 17 us
-//             (42 %), [2, 64, 1280] fp16 7.8 us; with a checkpoint [4, 16384, 512] fp16 48 us (55 %)
-//   backward  [2, 262144, 64] fp32 110 us (57 %), [8, 4096, 320] bf16 32 us (31 %), [4, 1024, 640] bf16 15 us;
-//             from a checkpoint [4, 65536, 256] bf16 121 us (43 %), [4, 16384, 512] fp16 67 us (39 %)
+//   forward   [4, 262144, 128] fp16 SiLU 127 us (65 %), [4, 65536, 320] bf16 SiLU 96 us (54 %), [8, 4096, 512] fp16 25 us
+//             (41 %), [3, 2961, 640] fp32 16 us (43 %), [2, 64, 1280] fp16 8.1 us; with a checkpoint [4, 16384, 512] fp16
+//             47 us (56 %)
+//   backward  [2, 262144, 64] fp32 113 us (55 %), [4, 65536, 320] bf16 165 us (47 %), [8, 4096, 320] bf16 32 us (31 %),
+//             [4, 1024, 640] bf16 15 us; from a checkpoint [4, 65536, 256] bf16 124 us (42 %), [4, 16384, 512] fp16 68 us (39 %)
 //
 // Split.  An item is a slice of an image's channels (whole groups and whole vectors, a 128-byte row or
 // more where the sizes allow it) over all its pixels.  A team of M thread blocks works on one item at a
@@ -34,8 +36,8 @@
 // consumer thread, the box of a 2-D tensor map over [batch * hw, channels]); the consumer warps wait on
 // a chunk's "full" mbarrier and release it through its "empty" one.  The ring runs on over the end of
 // a pass: while a block adds up its rows and waits for the others' sums, the first chunks of the next
-// pass are already under way.  The copies cost the consumers no issue slots, and those are what the
-// gradient runs short of first (per-thread cp.async into the same ring: 12 more instructions per vector).
+// pass are already under way.  The copies cost the consumers no instructions (per-thread cp.async into the same ring: 12
+// more per vector).
 //
 // Exchange outside clusters.  A block writes its sums per group to the workspace and counts itself in (the counters are
 // zeroed by a small kernel in front); before pass A one thread of a block polls the count, then

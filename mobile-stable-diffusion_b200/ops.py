@@ -3,6 +3,10 @@
 torch is used for device memory and streams only; every operation below is one call into
 libsdfl.so.  Inputs must be contiguous CUDA tensors of dtype float32 or float16 (the channels-last
 GroupNorm and the checkpoint functions also take bfloat16); gamma / beta are float32.  Nothing here computes on the host and nothing falls back to torch operators.
+
+torch.autograd does not see these calls: a result has no graph, whether or not an input requires grad.  Whoever
+trains with autograd calls a forward and a *_backward function from the two halves of a torch.autograd.Function,
+which keeps the statistics and the source (a tensor or a Checkpoint8) in between.
 """
 from __future__ import annotations
 

@@ -3,9 +3,11 @@ gradients.
 
 Bounds.  U = 2^-24 is half a step of fp32.  A result stored in type t is off by at most half a step of t
 (finfo(t).eps / 2 relative, or half the smallest subnormal) on top of the fp32 arithmetic, which is counted as
-K roundings of the terms it adds up: sums over n elements run in trees (at most 20 levels for 2^20 rows)
-after sequential runs of at most 32 elements in a thread, and an expression per element takes fewer
-than 12 operations, so K = 64.
+K roundings of the terms it adds up.  A thread adds up its rows one after another, 136 at most in the shapes that
+are tested here (hw / (thread blocks of a team * rows of threads) in general); the roundings of such a run have either
+sign, so n of them come to about sqrt(n), 12 here.  Trees over threads, blocks and channels have 20 levels at most,
+and an expression per element takes fewer than 12 operations: 44 in all, K = 64.  It is a bound for rounding
+errors as they occur, not for all of them at their largest with one sign.
 """
 from __future__ import annotations
 
