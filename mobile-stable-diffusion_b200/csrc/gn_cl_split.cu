@@ -3,8 +3,8 @@
 // gradient).  Formulas and layout: gn_cl_device.cuh.
 //
 // The form that takes every shape: channel counts that are not whole vectors, unaligned buffers, groups wider than
-// half a block's columns, and devices that do not hold a team's blocks at once.  Forward reads x twice and writes y, backward reads x and grad_out twice and writes
-// grad_x; the second read comes from L2 while the tensor fits it.  With whole vectors it takes 240 us where
+// half a block's columns, and devices that do not hold a team's blocks at once.  Forward reads x twice and writes y,
+// backward reads x and grad_out twice and writes grad_x; the second read comes from L2 while the tensor fits it.  With whole vectors it takes 240 us where
 // the single launch of gn_cl_team.cu takes 127 ([4, 262144, 128] fp16); [4, 16384, 1032] fp16 in 8 groups, which has no other,
 // takes 270 us (16 % of the measured copy bandwidth).
 #include "gn_cl_device.cuh"

@@ -82,7 +82,7 @@ constexpr int64_t kInFlight = 72ll << 20;          // twice that in the backward
 constexpr int kMaxCluster = 8;
 constexpr size_t kMaxShared = 200 * 1024;
 constexpr int64_t kSmShared = 228 * 1024;          // of an SM
-constexpr size_t kTwoOnSm = kSmShared / 3;          // staggered teams number their blocks by two on every SM: a third has no room
+constexpr size_t kTwoOnSm = kSmShared / 3;         // staggered teams number their blocks by two on every SM: no room for a third
 constexpr int64_t kBlockShared = 1024 + 128;       // that a block takes besides its dynamic shared memory: reserved, static
 constexpr int64_t kClusterPartBytes = 4096;        // shared memory for a cluster's sums
 constexpr int kMaxTeamsOfSm = kBlocksPerSm;        // teams that take turns on the SMs
@@ -1120,7 +1120,8 @@ cudaError_t launch(const Args &a, size_t smem, cudaStream_t stream, const Maps &
         int blocks = 0;
         err = blocks_of_sm<kernel>(dev, smem, &blocks);
         if (err != cudaSuccess) return err;
-        if (grid > static_cast<int64_t>(blocks) * sm_count() || (a.p.stagger && blocks != kMaxTeamsOfSm)) return cudaErrorCooperativeLaunchTooLarge;
+        if (grid > static_cast<int64_t>(blocks) * sm_count() || (a.p.stagger && blocks != kMaxTeamsOfSm))
+            return cudaErrorCooperativeLaunchTooLarge;
         const long long words = a.items + (a.p.stagger ? kSlotWords : 0);
         cl_clear_kernel<<<static_cast<unsigned>(std::min<long long>((words + 255) / 256, 256)), 256, 0, stream>>>(a.arrived, words);
         err = cudaGetLastError();
